@@ -225,6 +225,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     asm volatile("bar.sync 1, %0;\n" ::"n"(kThreads - 128) : "memory");      // the 384 threads that filled Q
   }
   const uint32_t tmem = sh->tmem_base;
+  // Completion of P.V(j).  Two query tiles: S(j + 1) of a tile is issued behind its P.V(j), so whoever has seen S(j) knows
+  // of every product up to P.V(j - 1) and one barrier per tile is unambiguous.  One query tile: Q.K^T runs two KV tiles
+  // ahead and seeing S(j) only tells of P.V(j - 2); a wait on the parity of P.V(j) alone would then pass while P.V(j - 1)
+  // is still running, so consecutive products take turns on two barriers.
+  auto pv_bar = [&](int t, int j) { return &sh->pv_done[kTiles == 2 ? t : (j & 1)]; };
+  auto pv_phase = [&](int j) { return (uint32_t)((kTiles == 2 ? j : (j >> 1)) & 1); };
 
   // Registers move from the loader / issue warpgroups (which need few) to the softmax warpgroups.
   // setmaxnreg.inc blocks until the CTA's register pool can satisfy it, and the pool is what the
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       }
       const float mu = m == -CUDART_INF_F ? 0.f : m;
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        alive = __all_sync(0xffffffffu, bar_wait(&sh->pv_done[t], (j - 1) & 1, &sh->abort));
+        alive = __all_sync(0xffffffffu, bar_wait(pv_bar(t, j - 1), pv_phase(j - 1), &sh->abort));
         if (!alive) break;
         tc_fence_after();
 #pragma unroll 1
@@ -358,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     }
     // epilogue: O / l -> bf16 rows of the output
     if (alive && my_tiles > 0) {
-      alive = __all_sync(0xffffffffu, bar_wait(&sh->pv_done[t], (my_tiles - 1) & 1, &sh->abort));
+      alive = __all_sync(0xffffffffu, bar_wait(pv_bar(t, my_tiles - 1), pv_phase(my_tiles - 1), &sh->abort));
       if (alive) {
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -485,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
         umma_bf16_ts_split(tmem + 256 + t * D, tmem + buf * 128 + k * 8, b + k * (2048 >> 4), v_hi, G_::kIdescPV,
                            (j > 0 || k > 0) ? 1u : 0u);
       }
-      umma_commit(&sh->pv_done[t]);
+      umma_commit(pv_bar(t, j));
     };
     if (kTiles == 1) {
       // One query tile, two score buffers: Q.K^T runs two KV tiles ahead of P.V, so the tensor pipe has the next
