@@ -40,6 +40,9 @@ _C = types.SimpleNamespace(
     _allocate_paged_slots_into=lambda last_slots, free_pages, prefixes, lengths, page_size, mapping, batch_requests:
         torch.ops.gaudirt._allocate_paged_slots_into(last_slots, free_pages, prefixes, lengths, page_size, mapping,
                                                      batch_requests),
+    _extend_paged_requests=lambda mapping, batch_requests, lengths, new_tokens, free_pages, used_pages, page_size, rows:
+        torch.ops.gaudirt._extend_paged_requests(mapping, batch_requests, lengths, new_tokens, free_pages, used_pages,
+                                                 page_size, rows),
     _release_paged_slots=lambda slots, page_size, max_pages:
         torch.ops.gaudirt._release_paged_slots(slots, page_size, max_pages),
 )
@@ -78,6 +81,20 @@ def _fake_paged_attn_validated(query, key, value, key_pool, value_pool, location
 @torch.library.register_fake("gaudirt::_paged_attn_stored")
 def _fake_paged_attn_stored(query, key_pool, value_pool, metadata, head_dim, scale, softcap=0.0, sliding_window=-1):
     return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+
+@torch.library.register_fake("gaudirt::_paged_attn_biased")
+def _fake_paged_attn_biased(query, key, value, key_pool, value_pool, metadata, slopes, head_dim, scale, softcap=0.0,
+                            sliding_window=-1):
+    return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+
+@torch.library.register_fake("gaudirt::_extend_paged_requests")
+def _fake_extend_paged_requests(mapping, batch_requests, lengths, new_tokens, free_pages, used_pages, page_size, rows):
+    torch._check(lengths.shape[0] == batch_requests.shape[0])
+    torch._check(lengths.shape[0] == new_tokens.shape[0])
+    return (*(batch_requests.new_empty(rows) for _ in range(3)), batch_requests.new_empty(lengths.shape[0] + 1),
+            torch.empty_like(lengths), torch.empty_like(used_pages))
 
 
 @torch.library.register_fake("gaudirt::_rotary_kv_store")

@@ -38,6 +38,16 @@ PROTOTYPES = {
     "gk_paged_attn_multi_bf16": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64, vp, i32, i64, vp, vp, vp, f32,
                                        f32, i32, i32, i32, i32, vp, vp]),
     "gk_paged_attn_combine_multi_bf16": (i32, [vp, vp, vp, i64, vp, i32, i64, i32, i32, vp]),
+    "gk_prefill_plan_build_two_way": (i32, [vp, i64, vp, i32, i32, i32, i32, vp, i64, i64p, vp, i64p]),
+    "gk_shared_prefix_plan_build": (i32, [vp, i64, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, i64, vp, i64, i64p,
+                                          vp, i64, i64p, i64p, vp, i64, i64p, vp, i64, i64p]),
+    "gk_shared_prefix_check": (i32, [vp, i64, i64, i64, vp, i64, vp, i64, vp, vp, vp]),
+    "gk_shared_prefix_attn_bf16": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64, vp, vp, vp, vp, f32, f32, i32,
+                                         i32, i32, i32, vp, vp]),
+    "gk_paged_attn_extended_multi_bf16": (i32, [vp, i64, vp, vp, i64, i64, vp, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64,
+                                                vp, i32, i64, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, vp, vp]),
+    "gk_paged_prefill_tc_biased_multi_bf16": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64, vp, i32, i64, vp,
+                                                    vp, f32, f32, i32, i32, i32, i32, vp, vp]),
     "gk_peer_barrier": (i32, [vp, i32, i32, i32, i64, vp, vp]),
     "gk_peer_barrier_counted": (i32, [vp, i32, i32, vp, i64, vp, vp]),
     "gk_rms_norm_bf16": (i32, [vp, vp, f32, f32, i64, i64, i64, vp, vp]),
@@ -49,6 +59,9 @@ PROTOTYPES = {
     "gk_paged_slots_allocate": (i32, [vp, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, vp, vp, vp, vp]),
     "gk_paged_slots_release_workspace_bytes": (i32, [i64, i64, C.POINTER(C.c_uint64)]),
     "gk_paged_slots_release": (i32, [vp, i64, i64, i64, vp, vp, vp, vp]),
+    "gk_extend_requests_workspace_bytes": (i32, [i64, C.POINTER(C.c_uint64)]),
+    "gk_extend_requests": (i32, [vp, i64, i64, i64, vp, vp, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp,
+                                 vp]),
     "gk_advance_decode_lengths": (i32, [vp, vp, i64, vp, vp, vp]),
     "gk_paged_metadata_device_workspace_bytes": (i32, [i64, C.POINTER(C.c_uint64)]),
     "gk_paged_metadata_device_validate": (i32, [vp, vp, vp, vp, i32, i64, vp, i64, i64, i64, i64, vp, i64, i64, vp,

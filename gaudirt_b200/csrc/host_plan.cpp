@@ -148,10 +148,24 @@ extern "C" int gk_paged_slots_layout(const int64_t* prefixes, const int64_t* len
   return GK_OK;
 }
 
-extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_heads, int kv_heads, int head_dim,
-                                       int window, int sm_count, int split_tokens, int32_t* work_out,
-                                       int64_t work_cap, int64_t* n_work_out, int32_t* combine_out,
-                                       int64_t combine_cap, int64_t* n_combine_out, int64_t* partial_entries_out) {
+namespace {
+// What a step may say about its sequences beyond their records (any pointer may be null):
+//   kv_from       first key of the sequence that its own work records cover (the keys before it are the shared
+//                 prefix, attended to elsewhere)
+//   parts_before  partial states of those keys that stand in front of the sequence's own splits
+//   two_way       keys below it are visible to every row of the sequence, not only to the rows behind them
+//   row_entry     out, [rows*2]: {first entry (query head 0), entries between two parts} of every row with parts_before
+struct SequenceExtras {
+  const int32_t* kv_from = nullptr;
+  const int32_t* parts_before = nullptr;
+  const int32_t* two_way = nullptr;
+  int32_t* row_entry = nullptr;
+};
+
+int attention_plan_build(const int32_t* seq, int64_t n_seq, const SequenceExtras& extras, int q_heads, int kv_heads,
+                         int head_dim, int window, int sm_count, int split_tokens, int32_t* work_out, int64_t work_cap,
+                         int64_t* n_work_out, int32_t* combine_out, int64_t combine_cap, int64_t* n_combine_out,
+                         int64_t* partial_entries_out) {
   if (!seq || n_seq <= 0 || !n_work_out || !n_combine_out || !partial_entries_out || sm_count <= 0 ||
       split_tokens < 0 || (window != -1 && window <= 0))
     return GK_ERR_INVALID_ARGUMENT;
@@ -161,18 +175,22 @@ extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_
   const int group = q_heads / kv_heads;
   const int block_rows = std::max(1, GK_MAX_PACKED_ROWS / group);
 
-  struct Block { int32_t first_row, n_rows, first_pos, table_row, lo, hi; };
+  struct Block { int32_t first_row, n_rows, first_pos, table_row, lo, hi, before; };
   std::vector<Block> blocks;
   int64_t total_span = 0;
   for (int64_t s = 0; s < n_seq; ++s) {
     const int32_t* r = seq + s * 4;
     if (r[1] <= 0 || r[2] < 0 || r[0] < 0 || r[3] < 0) return GK_ERR_INVALID_ARGUMENT;
+    const int32_t from = extras.kv_from ? extras.kv_from[s] : 0, before = extras.parts_before ? extras.parts_before[s] : 0;
+    const int32_t two_way = extras.two_way ? extras.two_way[s] : 0;
+    if (from < 0 || from > r[2] || before < 0 || two_way < 0 || (int64_t)two_way > (int64_t)r[2] + r[1])
+      return GK_ERR_INVALID_ARGUMENT;
     for (int32_t done = 0; done < r[1]; done += block_rows) {
       const int32_t n = std::min<int32_t>(block_rows, r[1] - done);
       const int64_t first_pos = (int64_t)r[2] + done;
       if (first_pos + n > INT32_MAX) return GK_ERR_UNSUPPORTED;
-      const int32_t lo = window > 0 ? (int32_t)std::max<int64_t>(0, first_pos - window + 1) : 0;
-      blocks.push_back({r[0] + done, n, (int32_t)first_pos, r[3], lo, (int32_t)(first_pos + n)});
+      const int32_t lo = std::max(from, window > 0 ? (int32_t)std::max<int64_t>(0, first_pos - window + 1) : 0);
+      blocks.push_back({r[0] + done, n, (int32_t)first_pos, r[3], lo, std::max((int32_t)(first_pos + n), two_way), before});
       total_span += blocks.back().hi - lo;
     }
   }
@@ -213,7 +231,7 @@ extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_
   thread_local Memo memo;
   uint64_t key = 1469598103934665603ull;
   auto mix = [&key](uint64_t v) { key = (key ^ v) * 1099511628211ull; };
-  for (const Block& b : blocks) { mix((uint64_t)b.n_rows << 32 | (uint32_t)b.lo); mix((uint32_t)b.hi); }
+  for (const Block& b : blocks) { mix((uint64_t)b.n_rows << 32 | (uint32_t)b.lo); mix((uint64_t)b.before << 32 | (uint32_t)b.hi); }
   mix(q_heads); mix(kv_heads); mix(head_dim); mix((uint32_t)window); mix(sm_count);
   if (chunk == 0 && memo.key == key && memo.chunk > 0) {
     chunk = memo.chunk;
@@ -311,13 +329,19 @@ extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_
     const int64_t span = b.hi - b.lo;
     int64_t splits, per;
     cut(span, chunk, uneven, splits, per);
-    if (splits > 0x7fff) return GK_ERR_CAPACITY;     // the split index shares a record word with the count
+    const int64_t parts = b.before + splits;         // states to merge: the ones in front, then the block's own splits
+    if (parts > 0x7fff) return GK_ERR_CAPACITY;      // the split index shares a record word with the count
     int64_t base = -1;
-    if (splits > 1) {
+    if (parts > 1) {
       base = entries;
-      entries += splits * b.n_rows * q_heads;
+      entries += parts * b.n_rows * q_heads;
       if (entries > INT32_MAX) return GK_ERR_CAPACITY;
-      merges.push_back({b.first_row, b.n_rows, (int32_t)base, (int32_t)splits});
+      merges.push_back({b.first_row, b.n_rows, (int32_t)base, (int32_t)parts});
+      if (b.before > 0 && extras.row_entry)
+        for (int32_t r = 0; r < b.n_rows; ++r) {
+          extras.row_entry[2 * (int64_t)(b.first_row + r)] = (int32_t)(base + (int64_t)r * q_heads);
+          extras.row_entry[2 * (int64_t)(b.first_row + r) + 1] = b.n_rows * q_heads;
+        }
     }
     for (int64_t s = 0; s < splits; ++s) {
       Item it{};
@@ -327,8 +351,9 @@ extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_
       it.w[3] = b.table_row;
       it.w[4] = (int32_t)(b.lo + s * per);
       it.w[5] = s + 1 == splits ? b.hi : (int32_t)(b.lo + (s + 1) * per);
-      it.w[6] = base < 0 ? -1 : (int32_t)(base + s * b.n_rows * q_heads);
-      it.w[7] = (int32_t)(splits | (s << 16));     // low half: splits of the block, high half: which one
+      const int64_t part = b.before + s;
+      it.w[6] = base < 0 ? -1 : (int32_t)(base + part * b.n_rows * q_heads);
+      it.w[7] = (int32_t)(parts | (part << 16));   // low half: states of the block to merge, high half: which one
       items.push_back(it);
     }
   }
@@ -346,9 +371,164 @@ extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_
   return GK_OK;
 }
 
-extern "C" int gk_prefill_plan_build(const int32_t* seq, int64_t n_seq, int q_heads, int kv_heads, int window,
-                                     int min_rows, int32_t* work_out, int64_t work_cap, int64_t* n_work_out,
-                                     int32_t* rest_seq_out, int64_t* n_rest_out) {
+}  // namespace
+
+extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_heads, int kv_heads, int head_dim,
+                                       int window, int sm_count, int split_tokens, int32_t* work_out,
+                                       int64_t work_cap, int64_t* n_work_out, int32_t* combine_out,
+                                       int64_t combine_cap, int64_t* n_combine_out, int64_t* partial_entries_out) {
+  return attention_plan_build(seq, n_seq, SequenceExtras{}, q_heads, kv_heads, head_dim, window, sm_count, split_tokens,
+                              work_out, work_cap, n_work_out, combine_out, combine_cap, n_combine_out, partial_entries_out);
+}
+
+// Sequences whose rows see a two-way prefix and, by group, read a common prefix together.
+extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, const int32_t* two_way, const int32_t* groups,
+                                           const int32_t* prefix_tokens, int64_t n_groups, int q_heads, int kv_heads,
+                                           int head_dim, int window, int sm_count, int split_tokens,
+                                           int prefix_split_tokens, int64_t min_saved_bytes, int32_t* work_out,
+                                           int64_t work_cap, int64_t* n_work_out, int32_t* combine_out,
+                                           int64_t combine_cap, int64_t* n_combine_out, int64_t* partial_entries_out,
+                                           int32_t* prefix_work_out, int64_t prefix_work_cap, int64_t* n_prefix_work_out,
+                                           int32_t* prefix_rows_out, int64_t prefix_rows_cap, int64_t* n_prefix_rows_out) {
+  if (!seq || n_seq <= 0 || n_groups < 0 || (n_groups > 0 && (!groups || !prefix_tokens)) || prefix_split_tokens < 0 ||
+      min_saved_bytes < 0 || !n_prefix_work_out || !n_prefix_rows_out || sm_count <= 0 || (window != -1 && window <= 0))
+    return GK_ERR_INVALID_ARGUMENT;
+  if (q_heads <= 0 || q_heads > 256 || kv_heads <= 0 || kv_heads > 256 || q_heads % kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256) || q_heads / kv_heads > GK_MAX_PACKED_ROWS)
+    return GK_ERR_UNSUPPORTED;
+  const int group_heads = q_heads / kv_heads;
+  const int tile = head_dim == 256 ? 64 : 128;                                    // keys of one tile of the kernel
+  const int record_rows = GK_PREFILL_TILES_PER_ITEM * (GK_PREFILL_TILE_ROWS / group_heads);
+  const int ctas_per_record = head_dim == 256 ? 2 : 1;
+
+  struct Group { std::vector<int32_t> members; int64_t rows = 0; int32_t lo = 0, hi = 0; };
+  std::vector<Group> all(static_cast<size_t>(n_groups));
+  int64_t last_row = 0;
+  for (int64_t s = 0; s < n_seq; ++s) {
+    const int32_t* r = seq + s * 4;
+    if (r[1] <= 0 || r[2] < 0 || r[0] < 0 || r[3] < 0 || (int64_t)r[2] + r[1] > INT32_MAX) return GK_ERR_INVALID_ARGUMENT;
+    last_row = std::max<int64_t>(last_row, (int64_t)r[0] + r[1]);
+    const int32_t g = n_groups > 0 ? groups[s] : -1;
+    if (g < -1 || g >= n_groups) return GK_ERR_INVALID_ARGUMENT;
+    if (g < 0) continue;
+    if (prefix_tokens[g] < 0 || prefix_tokens[g] > r[2]) return GK_ERR_INVALID_ARGUMENT;   // every row is behind the prefix
+    all[g].members.push_back((int32_t)s);
+    all[g].rows += r[1];
+  }
+  // A group is attended to together when that saves enough reading to pay for the launch and for the merge of its parts.
+  std::vector<Group*> shared;
+  const int64_t token_bytes = (int64_t)kv_heads * head_dim * 4;
+  for (int64_t g = 0; g < n_groups; ++g) {
+    Group& one = all[g];
+    one.hi = prefix_tokens[g];
+    one.lo = one.hi;
+    for (int32_t s : one.members)
+      one.lo = std::min(one.lo, window > 0 ? std::max(0, seq[s * 4 + 2] - window + 1) : 0);   // first key any row sees
+    if (one.members.size() < 2 || one.hi <= one.lo) continue;
+    one.lo = one.lo / tile * tile;                                   // whole tiles: a row's own window is masked in the kernel
+    if ((int64_t)(one.members.size() - 1) * (one.hi - one.lo) * token_bytes < min_saved_bytes) continue;
+    shared.push_back(&one);
+  }
+  // How long a piece of the prefix one CTA takes: the cheapest of the whole-tile lengths, by the time the CTAs need on
+  // sm_count SMs (one CTA each), in units of one key tile against two query tiles.  A CTA costs its tiles and a fixed
+  // prologue and epilogue; every piece leaves (m, l, O) states that are written and read once more.
+  int64_t piece = prefix_split_tokens;
+  if (piece == 0 && !shared.empty()) {
+    int32_t longest = 0;
+    for (const Group* g : shared) longest = std::max(longest, g->hi - g->lo);
+    constexpr double kCtaTiles = 2.5, kStateTiles = 0.2;
+    double best = 0.0;
+    for (int64_t tiles = 1; tiles <= (longest + tile - 1) / tile; tiles = tiles < 16 ? tiles + 1 : tiles + tiles / 8) {
+      std::vector<int32_t> costs;                                 // tiles per CTA; the scheduler takes them in order
+      double states = 0.0;
+      for (const Group* g : shared) {
+        const int64_t records = (g->rows + record_rows - 1) / record_rows * kv_heads * ctas_per_record;
+        const int64_t span = (g->hi - g->lo + tile - 1) / tile, pieces = (span + tiles - 1) / tiles;
+        const int64_t even = (span + pieces - 1) / pieces;
+        states += (double)(pieces * records);
+        if (pieces * records > 16 * (int64_t)sm_count) { costs.clear(); break; }
+        for (int64_t i = 0; i < pieces; ++i)
+          for (int64_t k = 0; k < records; ++k) costs.push_back((int32_t)std::min<int64_t>(even, span - i * even));
+      }
+      if (costs.empty()) {
+        if (tiles < (longest + tile - 1) / tile) continue;
+        piece = tiles * tile;                                     // many CTAs whatever the cut: no cut at all
+        break;
+      }
+      std::sort(costs.begin(), costs.end(), std::greater<int32_t>());
+      std::vector<double> heap((size_t)sm_count, 0.0);
+      auto later = std::greater<double>();
+      double makespan = 0.0;
+      for (int32_t c : costs) {
+        std::pop_heap(heap.begin(), heap.end(), later);
+        heap.back() += c + kCtaTiles;
+        makespan = std::max(makespan, heap.back());
+        std::push_heap(heap.begin(), heap.end(), later);
+      }
+      const double cost = makespan + kStateTiles * states / sm_count;
+      if (piece == 0 || cost < best) {
+        best = cost;
+        piece = tiles * tile;
+      }
+    }
+  }
+  if (piece > 0) piece = round_up(std::max<int64_t>(piece, tile), tile);
+
+  std::vector<int32_t> kv_from(static_cast<size_t>(n_seq), 0), before(static_cast<size_t>(n_seq), 0);
+  struct Item { int32_t w[GK_WORK_WORDS]; };
+  std::vector<Item> items;
+  std::vector<std::array<int32_t, 4>> rows;
+  for (const Group* g : shared) {
+    const int64_t span = (g->hi - g->lo + tile - 1) / tile, pieces = (span * tile + piece - 1) / piece;
+    const int64_t even = (span + pieces - 1) / pieces * tile, parts = (span * tile + even - 1) / even;
+    if (parts >= 0x7fff) return GK_ERR_CAPACITY;
+    std::vector<std::array<int32_t, 2>> places;                   // {row, position}
+    for (int32_t s : g->members) {
+      kv_from[s] = g->hi;
+      before[s] = (int32_t)parts;
+      for (int32_t r = 0; r < seq[s * 4 + 1]; ++r) places.push_back({seq[s * 4] + r, seq[s * 4 + 2] + r});
+    }
+    for (size_t at = 0; at < places.size(); at += record_rows) {
+      const int32_t n = (int32_t)std::min<size_t>(record_rows, places.size() - at);
+      int32_t highest = 0;
+      for (int32_t i = 0; i < n; ++i) highest = std::max(highest, places[at + i][1]);
+      for (int64_t part = 0; part < parts; ++part)
+        items.push_back({{(int32_t)(rows.size()), n, (int32_t)part, seq[g->members[0] * 4 + 3], (int32_t)(g->lo + part * even),
+                          (int32_t)std::min<int64_t>(g->hi, g->lo + (part + 1) * even), highest, 0}});
+      for (int32_t i = 0; i < n; ++i) rows.push_back({places[at + i][0], places[at + i][1], 0, 0});
+    }
+  }
+  std::vector<int32_t> row_entry(static_cast<size_t>(last_row) * 2, 0);
+  SequenceExtras extras;
+  extras.kv_from = kv_from.data();
+  extras.parts_before = before.data();
+  extras.two_way = two_way;
+  extras.row_entry = row_entry.data();
+  const int built = attention_plan_build(seq, n_seq, extras, q_heads, kv_heads, head_dim, window, sm_count, split_tokens,
+                                         work_out, work_cap, n_work_out, combine_out, combine_cap, n_combine_out,
+                                         partial_entries_out);
+  if (built != GK_OK) return built;
+  *n_prefix_work_out = (int64_t)items.size();
+  *n_prefix_rows_out = (int64_t)rows.size();
+  if (!work_out) return GK_OK;
+  if (prefix_work_cap < (int64_t)items.size() || prefix_rows_cap < (int64_t)rows.size() ||
+      (!items.empty() && (!prefix_work_out || !prefix_rows_out)))
+    return GK_ERR_CAPACITY;
+  std::stable_sort(items.begin(), items.end(),
+                   [](const Item& a, const Item& b) { return a.w[5] - a.w[4] > b.w[5] - b.w[4]; });
+  for (size_t i = 0; i < items.size(); ++i) std::copy(items[i].w, items[i].w + GK_WORK_WORDS, prefix_work_out + i * GK_WORK_WORDS);
+  for (size_t i = 0; i < rows.size(); ++i) {
+    rows[i][2] = row_entry[2 * (size_t)rows[i][0]];
+    rows[i][3] = row_entry[2 * (size_t)rows[i][0] + 1];
+    std::copy(rows[i].begin(), rows[i].end(), prefix_rows_out + i * 4);
+  }
+  return GK_OK;
+}
+
+namespace {
+int prefill_plan_build(const int32_t* seq, int64_t n_seq, const int32_t* two_way, int q_heads, int kv_heads, int window,
+                       int min_rows, int32_t* work_out, int64_t work_cap, int64_t* n_work_out, int32_t* rest_seq_out,
+                       int64_t* n_rest_out) {
   if (!seq || n_seq <= 0 || !n_work_out || !n_rest_out || min_rows < 0 || (window != -1 && window <= 0))
     return GK_ERR_INVALID_ARGUMENT;
   if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || q_heads / kv_heads > GK_PREFILL_TILE_ROWS)
@@ -363,6 +543,7 @@ extern "C" int gk_prefill_plan_build(const int32_t* seq, int64_t n_seq, int q_he
   for (int64_t s = 0; s < n_seq; ++s) {
     const int32_t* r = seq + s * 4;
     if (r[1] <= 0 || r[2] < 0 || r[0] < 0 || r[3] < 0) return GK_ERR_INVALID_ARGUMENT;
+    if (two_way && (two_way[s] < 0 || (int64_t)two_way[s] > (int64_t)r[2] + r[1])) return GK_ERR_INVALID_ARGUMENT;
     if (r[1] < min_rows) {
       if (rest_seq_out) std::copy(r, r + 4, rest_seq_out + n_rest * 4);
       ++n_rest;
@@ -378,7 +559,7 @@ extern "C" int gk_prefill_plan_build(const int32_t* seq, int64_t n_seq, int q_he
       it.w[2] = (int32_t)first_pos;
       it.w[3] = r[3];
       it.w[4] = window > 0 ? (int32_t)std::max<int64_t>(0, first_pos - window + 1) : 0;
-      it.w[5] = (int32_t)(first_pos + n);
+      it.w[5] = std::max((int32_t)(first_pos + n), two_way ? two_way[s] : 0);
       it.w[6] = -1;
       it.w[7] = 1;
       items.push_back(it);
@@ -392,4 +573,19 @@ extern "C" int gk_prefill_plan_build(const int32_t* seq, int64_t n_seq, int q_he
                    [](const Item& a, const Item& b) { return a.w[5] - a.w[4] > b.w[5] - b.w[4]; });
   for (size_t i = 0; i < items.size(); ++i) std::copy(items[i].w, items[i].w + GK_WORK_WORDS, work_out + i * GK_WORK_WORDS);
   return GK_OK;
+}
+}  // namespace
+
+extern "C" int gk_prefill_plan_build(const int32_t* seq, int64_t n_seq, int q_heads, int kv_heads, int window,
+                                     int min_rows, int32_t* work_out, int64_t work_cap, int64_t* n_work_out,
+                                     int32_t* rest_seq_out, int64_t* n_rest_out) {
+  return prefill_plan_build(seq, n_seq, nullptr, q_heads, kv_heads, window, min_rows, work_out, work_cap, n_work_out,
+                            rest_seq_out, n_rest_out);
+}
+
+extern "C" int gk_prefill_plan_build_two_way(const int32_t* seq, int64_t n_seq, const int32_t* two_way, int q_heads,
+                                             int kv_heads, int window, int min_rows, int32_t* work_out, int64_t work_cap,
+                                             int64_t* n_work_out, int32_t* rest_seq_out, int64_t* n_rest_out) {
+  return prefill_plan_build(seq, n_seq, two_way, q_heads, kv_heads, window, min_rows, work_out, work_cap, n_work_out,
+                            rest_seq_out, n_rest_out);
 }

@@ -122,8 +122,51 @@ __global__ void prefix_kernel(const RowArgs a) {
   }
 }
 
+// Table rows that are declared to begin alike: grid (pairs, chunks), pairs[i] = {row of the group's first member, row of
+// another member, tokens, sequence}.  `verdict` receives the smallest sequence that differs (all ones: none).
+__global__ void shared_tables_kernel(const int32_t* __restrict__ table, int64_t n_requests, int64_t context,
+                                     int64_t table_stride, const int32_t* __restrict__ table_rows, int64_t n_table_rows,
+                                     const int4* __restrict__ pairs, unsigned* verdict, int32_t* status) {
+  const int4 pair = pairs[blockIdx.x];
+  auto row_of = [&](int index) -> int64_t {
+    if (index < 0 || index >= n_table_rows) return -1;
+    const int64_t row = table_rows ? table_rows[index] : index;
+    return row >= 0 && row < n_requests ? row : -1;
+  };
+  const int64_t first = row_of(pair.x), other = row_of(pair.y);
+  bool differs = first < 0 || other < 0 || pair.z > context;
+  if (!differs && first != other)
+    for (int64_t p = (int64_t)blockIdx.y * blockDim.x + threadIdx.x; p < pair.z; p += (int64_t)gridDim.y * blockDim.x)
+      differs |= table[first * table_stride + p] != table[other * table_stride + p];
+  if (__syncthreads_or(differs) && threadIdx.x == 0) {
+    atomicMin(verdict, (unsigned)pair.w);
+    if (status) atomicOr(status, (int)GK_DEV_BAD_METADATA);
+  }
+}
+
 }  // namespace
 }  // namespace gk
+
+extern "C" int gk_shared_prefix_check(const int32_t* table, int64_t n_requests, int64_t context, int64_t table_stride,
+                                      const int32_t* table_rows, int64_t n_table_rows, const int32_t* pairs,
+                                      int64_t n_pairs, int32_t* verdict, int32_t* status, gk_stream_t stream) {
+  using namespace gk;
+  if (n_pairs == 0) return GK_OK;
+  if (!table || !pairs || !verdict || n_requests <= 0 || context <= 0 || context > INT32_MAX || table_stride < context ||
+      n_table_rows <= 0 || n_pairs < 0 || n_pairs > INT32_MAX || (reinterpret_cast<uintptr_t>(pairs) & 15))
+    return GK_ERR_INVALID_ARGUMENT;
+  auto s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = cudaMemsetAsync(verdict, 0xFF, sizeof(int32_t), s);
+  if (e != cudaSuccess) {
+    g_last_cuda_error = (int)e;
+    return GK_ERR_CUDA;
+  }
+  const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((context + kPrefixChunk - 1) / kPrefixChunk, 1184 / n_pairs));
+  shared_tables_kernel<<<dim3((unsigned)n_pairs, (unsigned)chunks), kThreads, 0, s>>>(
+      table, n_requests, context, table_stride, table_rows, n_table_rows, reinterpret_cast<const int4*>(pairs),
+      reinterpret_cast<unsigned*>(verdict), status);
+  return check_launch();
+}
 
 extern "C" int gk_paged_metadata_device_workspace_bytes(int64_t slots, uint64_t* bytes_out) {
   if (!bytes_out || slots <= 0 || slots > INT32_MAX) return GK_ERR_INVALID_ARGUMENT;

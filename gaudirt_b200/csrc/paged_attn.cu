@@ -56,6 +56,10 @@ struct AttnParams {
   int64_t part_capacity;                 // entries part_ml / part_o hold; a record that points past it is skipped
   float scale, softcap;
   int window, page_shift, q_heads, kv_heads, group, n_out;
+  // read by the extended form only (template argument EXT), each may be null:
+  const float* slopes;                   // [q_heads]: the score of key j gets -slope * |position - j|
+  const int32_t* row_limits;             // [rows]: last key a row sees, at or behind its position (two-way prefix)
+  const int32_t* parts_before;           // [rows]: states of a shared prefix that stand in front of the block's own splits
 };
 
 template <int D, int WARPS, int STAGES>
@@ -80,7 +84,8 @@ __device__ __forceinline__ uint32_t group_off(int row, int chunk) {
   return (chunk >> 3) * (kGroupTokens * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
-template <int D, int WARPS, int STAGES, bool TMA>
+// EXT: distance bias, row limits and states of a shared prefix; without it none of the three costs an instruction.
+template <int D, int WARPS, int STAGES, bool TMA, bool EXT>
 __global__ void __launch_bounds__(WARPS * 32, 2) paged_attn_kernel(const AttnParams p,
                                                                    const __grid_constant__ CUtensorMap map_kv) {
   using C = AttnConfig<D, WARPS, STAGES>;
@@ -101,6 +106,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_attn_kernel(const AttnPar
   // ---- Q fragments (A operand of S = Q K^T), rows g and g+8 of the packed tile ----------
   uint32_t qf[D / 16][4];
   int lim0 = 0x7fffffff, lim1 = 0x7fffffff;                     // last visible key per row
+  int pos0 = 0x7fffffff, pos1 = 0x7fffffff;                     // the row's own position (EXT; otherwise its limit)
+  float slope0 = 0.f, slope1 = 0.f;                             // EXT: bias per token of distance, in log2 units
   {
     const unsigned short* q0 = nullptr;
     const unsigned short* q1 = nullptr;
@@ -109,12 +116,22 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_attn_kernel(const AttnPar
       lim0 = first_pos + r;
       q0 = reinterpret_cast<const unsigned short*>(p.q) + (int64_t)(first_row + r) * p.q_stride +
            (int64_t)(head * G + gq) * D;
+      if (EXT) {
+        pos0 = lim0;
+        if (p.row_limits) lim0 = __ldg(p.row_limits + first_row + r);
+        if (p.slopes) slope0 = __ldg(p.slopes + head * G + gq) * kLog2e;
+      }
     }
     if (g + 8 < mv) {
       const int r = (g + 8) / G, gq = g + 8 - r * G;
       lim1 = first_pos + r;
       q1 = reinterpret_cast<const unsigned short*>(p.q) + (int64_t)(first_row + r) * p.q_stride +
            (int64_t)(head * G + gq) * D;
+      if (EXT) {
+        pos1 = lim1;
+        if (p.row_limits) lim1 = __ldg(p.row_limits + first_row + r);
+        if (p.slopes) slope1 = __ldg(p.slopes + head * G + gq) * kLog2e;
+      }
     }
     // two consecutive bf16 of a query row: one 32-bit load when the row is 4-byte aligned (col is even), else
     // two 16-bit loads (the reference's one-element-offset views are only 2-byte aligned)
@@ -318,6 +335,15 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_attn_kernel(const AttnPar
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sc[nt][e] *= to_log2;
+    if (EXT && p.slopes) {
+      // -slope * |position - key|: the distance is taken in integers and rounded once (exact below 2^24)
+      const float d0 = (float)(tok0 + 2 * t - pos0), d1 = (float)(tok0 + 2 * t - pos1);
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sc[nt][e] = fmaf(e < 2 ? -slope0 : -slope1, fabsf((e < 2 ? d0 : d1) + (float)(nt * 8 + (e & 1))), sc[nt][e]);
+    }
     const bool ragged = tok0 + kGroupTokens > kv_end || tok0 + kGroupTokens > first_pos + 1 ||
                         (p.window > 0 && tok0 <= first_pos + n_rows - 1 - p.window);
     if (ragged) {
@@ -327,7 +353,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_attn_kernel(const AttnPar
         for (int e = 0; e < 4; ++e) {
           const int tok = tok0 + nt * 8 + 2 * t + (e & 1);
           const int lim = e < 2 ? lim0 : lim1;
-          const bool seen = tok < kv_end && tok <= lim && (p.window <= 0 || tok > lim - p.window);
+          const int pos = EXT ? (e < 2 ? pos0 : pos1) : lim;
+          const bool seen = tok < kv_end && tok <= lim && (p.window <= 0 || tok > pos - p.window);
           if (!seen) sc[nt][e] = -CUDART_INF_F;
         }
     }
@@ -471,7 +498,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) paged_attn_kernel(const AttnPar
     if (threadIdx.x == 0) {
       int* counter = p.counters + (int64_t)first_row * p.kv_heads + head;
       const int seen = atomicAdd(counter, 1);
-      is_last = seen == n_splits - 1;
+      // the states of a shared prefix are there already: their kernel ran before this one
+      const int before = EXT && p.parts_before ? __ldg(p.parts_before + first_row) : 0;
+      is_last = seen == n_splits - before - 1;
       if (is_last) *counter = 0;
     }
     __syncthreads();
@@ -601,10 +630,10 @@ __global__ void __launch_bounds__(128) paged_attn_combine_kernel(const float* __
 constexpr int kWarps = 4;
 constexpr int kStages = 3;
 
-template <int D, bool TMA>
+template <int D, bool TMA, bool EXT>
 int launch_attn_form(const AttnParams& p, const CUtensorMap& map_kv, int64_t n_work, cudaStream_t stream) {
   using C = AttnConfig<D, kWarps, kStages>;
-  auto kernel = paged_attn_kernel<D, kWarps, kStages, TMA>;
+  auto kernel = paged_attn_kernel<D, kWarps, kStages, TMA, EXT>;
   static std::atomic<bool> configured[64];
   const int ready = opt_in_shared_memory(kernel, C::kSmemBytes, configured);
   if (ready != GK_OK) return ready;
@@ -643,7 +672,11 @@ int launch_attn(const AttnParams& p, int64_t n_work, int page_tokens, cudaStream
                                                     : form == GK_ATTENTION_FORM_BOXES;
   const bool boxed = boxes && page_tokens >= kGroupTokens && pool_rows < 0x7fffffffLL &&
                      make_kv_group_map(&map_kv, p.pool_k, v_minus_k, pool_rows, kGroupTokens, D);
-  return boxed ? launch_attn_form<D, true>(p, map_kv, n_work, stream) : launch_attn_form<D, false>(p, map_kv, n_work, stream);
+  if (p.slopes || p.row_limits || p.parts_before)
+    return boxed ? launch_attn_form<D, true, true>(p, map_kv, n_work, stream)
+                 : launch_attn_form<D, false, true>(p, map_kv, n_work, stream);
+  return boxed ? launch_attn_form<D, true, false>(p, map_kv, n_work, stream)
+               : launch_attn_form<D, false, false>(p, map_kv, n_work, stream);
 }
 
 // Argument checks + launch of the attention kernel.  `part_capacity` is the number of entries the
@@ -654,8 +687,12 @@ int attn_entry(const void* q, int64_t q_row_stride, const void* pool_k, const vo
                int64_t out_row_stride, float* part_ml, float* part_o, int64_t part_capacity, int32_t* split_counters,
                float scale, float softcap, int window, int q_heads, int kv_heads, int head_dim, int32_t* status,
                gk_stream_t stream, const void* new_k = nullptr, const void* new_v = nullptr, int64_t new_k_stride = 0,
-               int64_t new_v_stride = 0, const int32_t* locations = nullptr) {
+               int64_t new_v_stride = 0, const int32_t* locations = nullptr, const float* slopes = nullptr,
+               const int32_t* row_limits = nullptr, const int32_t* parts_before = nullptr) {
   if (n_work == 0) return GK_OK;
+  if ((reinterpret_cast<uintptr_t>(slopes) | reinterpret_cast<uintptr_t>(row_limits) |
+       reinterpret_cast<uintptr_t>(parts_before)) & 3)
+    return GK_ERR_INVALID_ARGUMENT;
   if (new_k || new_v || locations) {
     // the fused store moves whole 16-byte pieces
     if (!new_k || !new_v || !locations || new_k_stride < (int64_t)kv_heads * head_dim ||
@@ -713,6 +750,9 @@ int attn_entry(const void* q, int64_t q_row_stride, const void* pool_k, const vo
   p.q_heads = q_heads;
   p.kv_heads = kv_heads;
   p.group = q_heads / kv_heads;
+  p.slopes = slopes;
+  p.row_limits = row_limits;
+  p.parts_before = parts_before;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (head_dim) {
     case 64: return launch_attn<64>(p, n_work, page_tokens, s);
@@ -750,6 +790,19 @@ extern "C" int gk_paged_attn_store_multi_bf16(const void* q, int64_t q_row_strid
                         table_rows, work, n_work, outs, n_outs, out_row_stride, part_ml, part_o, INT64_MAX,
                         split_counters, scale, softcap, window, q_heads, kv_heads, head_dim, status, stream, new_k, new_v,
                         new_k_row_stride, new_v_row_stride, locations);
+}
+
+extern "C" int gk_paged_attn_extended_multi_bf16(
+    const void* q, int64_t q_row_stride, const void* new_k, const void* new_v, int64_t new_k_row_stride,
+    int64_t new_v_row_stride, const int32_t* locations, void* pool_k, void* pool_v, int64_t slots, const int32_t* table,
+    int64_t table_stride, int64_t table_entry_stride, int page_tokens, const int32_t* table_rows, const int32_t* work,
+    int64_t n_work, void* const* outs, int n_outs, int64_t out_row_stride, float* part_ml, float* part_o,
+    int32_t* split_counters, const float* slopes, const int32_t* row_limits, const int32_t* parts_before, float scale,
+    float softcap, int window, int q_heads, int kv_heads, int head_dim, int32_t* status, gk_stream_t stream) {
+  return gk::attn_entry(q, q_row_stride, pool_k, pool_v, slots, table, table_stride, table_entry_stride, page_tokens,
+                        table_rows, work, n_work, outs, n_outs, out_row_stride, part_ml, part_o, INT64_MAX,
+                        split_counters, scale, softcap, window, q_heads, kv_heads, head_dim, status, stream, new_k, new_v,
+                        new_k_row_stride, new_v_row_stride, locations, slopes, row_limits, parts_before);
 }
 
 extern "C" int gk_paged_attn_bf16(const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v,

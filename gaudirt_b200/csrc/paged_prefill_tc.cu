@@ -80,6 +80,12 @@ struct PrefillParams {
   int window, page_shift, q_heads, kv_heads, group;
   int tma_rows;          // rows of a TMA box, 0 = TMA path off
   int n_out;
+  // read by the biased and the shared forms only (template arguments), the first two may be null:
+  const float* slopes;          // [q_heads]: the score of key j gets -slope * |position - j|
+  const int32_t* row_limits;    // [rows]: last key a row sees, at or behind its position (two-way prefix)
+  const int4* list;             // shared form: {row, position, first entry, entries between two parts} per listed row
+  float* part_ml;               // shared form: (m in log2 units, l) and un-normalised O of every entry
+  float* part_o;
 };
 
 struct Shared {
@@ -129,7 +135,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-template <int D>
+// BIASED: a distance bias and row limits.  SHARED: the rows of a record are listed (they belong to several sequences
+// that share the keys of the record), every listed row sees all of the record's keys but for its window, and the state
+// (m, l, O) is left for the merge instead of a normalised row.  A record of the shared form is {first listed row,
+// n_rows, part, table_row, kv_begin, kv_end, largest position, 0}.
+template <int D, bool BIASED, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const PrefillParams p,
                                                                        const __grid_constant__ CUtensorMap map_k,
                                                                        const __grid_constant__ CUtensorMap map_v) {
@@ -156,6 +166,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   const int4 w1 = __ldg(reinterpret_cast<const int4*>(p.work) + 2 * item + 1);
   const int G = p.group;
   const int tile_rows = kRows / G;                          // rows of the record per query tile
+  // last key that row `row`, at position `pos`, sees
+  auto last_seen = [&](int row, int pos) { return BIASED && p.row_limits ? __ldg(p.row_limits + row) : pos; };
   int first_row = w0.x, n_rows = w0.y, first_pos = w0.z, kv_begin = w1.x, kv_end = w1.y;
   const int table_row = w0.w;
   if (kTiles == 1) {                                        // this CTA's tile of the record, as a record of its own
@@ -163,14 +175,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     n_rows = min(n_rows - skip, tile_rows);
     if (n_rows <= 0) return;                                // the whole CTA: nothing is allocated yet
     first_row += skip;
-    first_pos += skip;
-    kv_end = min(kv_end, first_pos + n_rows);               // causal: nothing after this tile's last row
-    if (p.window > 0) kv_begin = max(kv_begin, first_pos - p.window + 1);
+    if (!SHARED) {
+      first_pos += skip;
+      kv_end = min(kv_end, last_seen(first_row + n_rows - 1, first_pos + n_rows - 1) + 1);   // causal: nothing after this tile's last row
+      if (p.window > 0) kv_begin = max(kv_begin, first_pos - p.window + 1);
+    }
   }
   const int rows0 = min(n_rows, tile_rows), rows1 = n_rows - rows0;
   // KV tiles each query tile needs: tile 0 stops at its own last row (causal), tile 1 at the record's end
   const int nt1_all = (kv_end - kv_begin + kKv - 1) / kKv;
-  const int nt0 = min(nt1_all, (first_pos + rows0 - kv_begin + kKv - 1) / kKv);
+  const int nt0 = SHARED ? nt1_all : min(nt1_all, (last_seen(first_row + rows0 - 1, first_pos + rows0 - 1) + 1 - kv_begin + kKv - 1) / kKv);
   const int nt1 = rows1 > 0 ? nt1_all : 0;
   const int n_tiles = max(nt0, nt1);
 
@@ -208,7 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       uint4 v = make_uint4(0, 0, 0, 0);
       const int r = t * tile_rows + pr / G, g = pr % G;
       if (pr < tile_rows * G && r < n_rows) {
-        const __nv_bfloat16* src = p.q + (int64_t)(first_row + r) * p.q_stride + (int64_t)(head * G + g) * D + c * 8;
+        const int row = SHARED ? __ldg(&p.list[first_row + r].x) : first_row + r;
+        const __nv_bfloat16* src = p.q + (int64_t)row * p.q_stride + (int64_t)(head * G + g) * D + c * 8;
         if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
           v = __ldg(reinterpret_cast<const uint4*>(src));
         } else {
@@ -252,7 +267,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     const int mv = my_rows * G;                                  // packed rows of this tile in use
     const int my_tiles = t == 0 ? nt0 : nt1;
     const int tile_first_pos = first_pos + t * tile_rows;
-    const int lim = pr < mv ? tile_first_pos + pr / G : 0x7fffffff;   // last visible key of this row
+    int lim = pr < mv ? tile_first_pos + pr / G : 0x7fffffff;         // last visible key of this row
+    int pos = lim;                                                     // its position
+    int4 listed = make_int4(0, 0, 0, 0);
+    if (SHARED) {
+      if (pr < mv) listed = __ldg(p.list + first_row + t * tile_rows + pr / G);
+      pos = pr < mv ? listed.y : 0x7fffffff;
+      lim = 0x7fffffff;
+    } else if (BIASED && pr < mv) {
+      lim = last_seen(first_row + t * tile_rows + pr / G, pos);
+    }
+    // bias per token of distance, in log2 units
+    const float slope = BIASED && p.slopes && pr < mv ? __ldg(p.slopes + head * G + pr % G) * kLog2e : 0.f;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + 256 + t * D + lane_base;
     const bool capped = p.softcap > 0.f;
@@ -272,8 +298,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       tc_fence_after();
       const int tok0 = kv_begin + j * kKv;
       const int tile_end = tok0 + kKv;
-      const bool ragged = tile_end > kv_end || tile_end > tile_first_pos + 1 ||
-                          (p.window > 0 && tok0 <= tile_first_pos + my_rows - 1 - p.window);
+      const bool ragged = SHARED ? tile_end > kv_end || (p.window > 0 && tok0 <= w1.z - p.window)
+                                 : tile_end > kv_end || tile_end > tile_first_pos + 1 ||
+                                       (p.window > 0 && tok0 <= tile_first_pos + my_rows - 1 - p.window);
+      const float from = BIASED ? (float)(tok0 - pos) : 0.f;      // key tok0 + e is at distance |from + e|
       // Softcap and tiles that need masking are uncommon: they first rewrite S in tensor memory (scores in
       // log2 units, masked keys at -inf), 32 columns at a time in a loop that is NOT unrolled, so that
       // the two passes below stay one short piece of code (the instruction cache is what this kernel
@@ -289,8 +317,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
             float v = __uint_as_float(r[e]);
             if (capped) v = p.softcap * tanhf(v * cap_in);
             v *= to_log2;
+            if (BIASED) v = fmaf(-slope, fabsf(from + (float)(c * 32 + e)), v);
             const int tok = tok0 + c * 32 + e;
-            const bool seen = tok < kv_end && tok <= lim && (p.window <= 0 || tok > lim - p.window);
+            const bool seen = tok < kv_end && tok <= lim && (p.window <= 0 || tok > pos - p.window);
             r[e] = __float_as_uint(seen ? v : -CUDART_INF_F);
           }
           tmem_st32(s_addr + c * 32, r);
@@ -302,6 +331,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
 #pragma unroll
       for (int c = 0; c < kScoreChunks; ++c) tmem_ld32_nowait(s_addr + c * 32, sr[c]);
       tmem_ld_wait();
+      if (BIASED && !(capped || ragged)) {
+        // every key of an unmasked tile is at or before the row's position: -slope * |distance| = slope * (from + e)
+        const float2 slope2 = make_float2(slope, slope), first2 = make_float2(slope * from, slope * from), mult_in = make_float2(mult, mult);
+#pragma unroll
+        for (int c = 0; c < kScoreChunks; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 bias = __ffma2_rn(slope2, make_float2((float)(c * 32 + e), (float)(c * 32 + e + 1)), first2);
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), mult_in, bias);
+            sr[c][e] = __float_as_uint(x.x);
+            sr[c][e + 1] = __float_as_uint(x.y);
+          }
+        mult = 1.f;
+      }
       float mx;
       {
         float part[kScoreChunks];
@@ -367,6 +410,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       alive = __all_sync(0xffffffffu, bar_wait(pv_bar(t, my_tiles - 1), pv_phase(my_tiles - 1), &sh->abort));
       if (alive) {
         tc_fence_after();
+        if (SHARED) {
+          const int64_t entry = (int64_t)listed.z + (int64_t)w0.z * listed.w + head * G + pr % G;
+          if (pr < mv) *reinterpret_cast<float2*>(p.part_ml + entry * 2) = make_float2(m, l);
+#pragma unroll 1
+          for (int cb = 0; cb < D / 32; ++cb) {
+            uint32_t r[32];
+            tmem_ld32(o_addr + cb * 32, r);
+            if (pr < mv) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(p.part_o + entry * D + cb * 32 + c * 4) = make_uint4(r[c * 4], r[c * 4 + 1], r[c * 4 + 2], r[c * 4 + 3]);
+            }
+          }
+        } else {
         const float inv = l > 0.f ? 1.f / l : 0.f;
         const int r_q = t * tile_rows + pr / G, g = pr % G;
         const int64_t at = (int64_t)(first_row + r_q) * p.out_stride + (int64_t)(head * G + g) * D;
@@ -385,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
               for (int dst = 0; dst < p.n_out; ++dst) *reinterpret_cast<uint4*>(p.out[dst] + at + cb * 32 + c * 8) = v;
             }
           }
+        }
         }
       }
     }
@@ -576,10 +634,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
 }
 
-template <int D>
+template <int D, bool BIASED, bool SHARED>
 int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream_t stream) {
   static std::atomic<bool> configured[64];
-  const int ready = opt_in_shared_memory(paged_prefill_tc_kernel<D>, Geo<D>::kSmemBytes, configured);
+  const int ready = opt_in_shared_memory(paged_prefill_tc_kernel<D, BIASED, SHARED>, Geo<D>::kSmemBytes, configured);
   if (ready != GK_OK) return ready;
   {
     // Never launch if the register pool of this build cannot satisfy the budgets (the kernel would hang).
@@ -587,7 +645,7 @@ int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream
     int regs = launch_regs.load(std::memory_order_acquire);
     if (regs < 0) {
       cudaFuncAttributes attr;
-      if (cudaFuncGetAttributes(&attr, paged_prefill_tc_kernel<D>) != cudaSuccess) return check_launch();
+      if (cudaFuncGetAttributes(&attr, paged_prefill_tc_kernel<D, BIASED, SHARED>) != cudaSuccess) return check_launch();
       regs = attr.numRegs;
       launch_regs.store(regs, std::memory_order_release);
     }
@@ -606,22 +664,40 @@ int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream
     p.tma_rows = box_rows;
   const int64_t ctas = n_work * p.kv_heads * (Geo<D>::kTiles == 2 ? 1 : 2);
   if (ctas > 0x7fffffffLL) return GK_ERR_UNSUPPORTED;
-  paged_prefill_tc_kernel<D><<<(unsigned)ctas, kThreads, Geo<D>::kSmemBytes, stream>>>(p, map_k, map_v);
+  paged_prefill_tc_kernel<D, BIASED, SHARED><<<(unsigned)ctas, kThreads, Geo<D>::kSmemBytes, stream>>>(p, map_k, map_v);
   return check_launch();
 }
 
-}  // namespace
-}  // namespace gk
 
-extern "C" int gk_paged_prefill_tc_multi_bf16(const void* q, int64_t q_row_stride, const void* pool_k,
-                                              const void* pool_v, int64_t slots, const int32_t* table,
-                                              int64_t table_stride, int64_t table_entry_stride, int page_tokens,
-                                              const int32_t* table_rows, const int32_t* work, int64_t n_work,
-                                              void* const* outs, int n_outs, int64_t out_row_stride, float scale,
-                                              float softcap, int window, int q_heads, int kv_heads, int head_dim,
-                                              int32_t* status, gk_stream_t stream) {
+// Which rows a launch of the kernel serves beyond its work records: a distance bias and row limits, or the listed rows of
+// the shared form with the split state that receives their part.
+struct PrefillExtras {
+  const float* slopes = nullptr;
+  const int32_t* row_limits = nullptr;
+  const int32_t* list = nullptr;
+  float* part_ml = nullptr;
+  float* part_o = nullptr;
+};
+
+template <bool BIASED, bool SHARED>
+int launch_prefill_dim(PrefillParams& p, int head_dim, int64_t n_work, int page_tokens, cudaStream_t stream) {
+  if (head_dim == 64) return launch_prefill<64, BIASED, SHARED>(p, n_work, page_tokens, stream);
+  if (head_dim == 256) return launch_prefill<256, BIASED, SHARED>(p, n_work, page_tokens, stream);
+  return launch_prefill<128, BIASED, SHARED>(p, n_work, page_tokens, stream);
+}
+
+int prefill_entry(const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v, int64_t slots,
+                  const int32_t* table, int64_t table_stride, int64_t table_entry_stride, int page_tokens,
+                  const int32_t* table_rows, const int32_t* work, int64_t n_work, void* const* outs, int n_outs,
+                  int64_t out_row_stride, const PrefillExtras& extras, float scale, float softcap, int window, int q_heads,
+                  int kv_heads, int head_dim, int32_t* status, gk_stream_t stream) {
   if (n_work == 0) return GK_OK;
-  if (!outs || n_outs <= 0 || n_outs > GK_MAX_OUTPUTS) return GK_ERR_INVALID_ARGUMENT;
+  const bool shared = extras.list != nullptr;
+  if (shared ? !extras.part_ml || !extras.part_o : !outs || n_outs <= 0 || n_outs > GK_MAX_OUTPUTS) return GK_ERR_INVALID_ARGUMENT;
+  if (((reinterpret_cast<uintptr_t>(extras.list) | reinterpret_cast<uintptr_t>(extras.part_o)) & 15) ||
+      (reinterpret_cast<uintptr_t>(extras.part_ml) & 7) ||
+      ((reinterpret_cast<uintptr_t>(extras.slopes) | reinterpret_cast<uintptr_t>(extras.row_limits)) & 3))
+    return GK_ERR_INVALID_ARGUMENT;
   for (int i = 0; i < n_outs; ++i)
     if (!outs[i] || (reinterpret_cast<uintptr_t>(outs[i]) & 15)) return GK_ERR_INVALID_ARGUMENT;
   if (!q || !pool_k || !pool_v || !table || !work || n_work < 0 || slots <= 0 || table_stride < 0 ||
@@ -634,7 +710,7 @@ extern "C" int gk_paged_prefill_tc_multi_bf16(const void* q, int64_t q_row_strid
   if (((reinterpret_cast<uintptr_t>(pool_k) | reinterpret_cast<uintptr_t>(pool_v) | reinterpret_cast<uintptr_t>(work)) & 15) ||
       (out_row_stride & 7) || (reinterpret_cast<uintptr_t>(q) & 1))
     return GK_ERR_INVALID_ARGUMENT;
-  gk::PrefillParams p{};
+  PrefillParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.pool_k = static_cast<const __nv_bfloat16*>(pool_k);
   p.pool_v = static_cast<const __nv_bfloat16*>(pool_v);
@@ -656,10 +732,68 @@ extern "C" int gk_paged_prefill_tc_multi_bf16(const void* q, int64_t q_row_strid
   p.q_heads = q_heads;
   p.kv_heads = kv_heads;
   p.group = q_heads / kv_heads;
+  p.slopes = extras.slopes;
+  p.row_limits = extras.row_limits;
+  p.list = reinterpret_cast<const int4*>(extras.list);
+  p.part_ml = extras.part_ml;
+  p.part_o = extras.part_o;
   cudaStream_t at = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 64) return gk::launch_prefill<64>(p, n_work, page_tokens, at);
-  if (head_dim == 256) return gk::launch_prefill<256>(p, n_work, page_tokens, at);
-  return gk::launch_prefill<128>(p, n_work, page_tokens, at);
+  if (shared)
+    return p.slopes ? launch_prefill_dim<true, true>(p, head_dim, n_work, page_tokens, at)
+                    : launch_prefill_dim<false, true>(p, head_dim, n_work, page_tokens, at);
+  return p.slopes || p.row_limits ? launch_prefill_dim<true, false>(p, head_dim, n_work, page_tokens, at)
+                                  : launch_prefill_dim<false, false>(p, head_dim, n_work, page_tokens, at);
+}
+
+}  // namespace
+}  // namespace gk
+
+extern "C" int gk_paged_prefill_tc_multi_bf16(const void* q, int64_t q_row_stride, const void* pool_k,
+                                              const void* pool_v, int64_t slots, const int32_t* table,
+                                              int64_t table_stride, int64_t table_entry_stride, int page_tokens,
+                                              const int32_t* table_rows, const int32_t* work, int64_t n_work,
+                                              void* const* outs, int n_outs, int64_t out_row_stride, float scale,
+                                              float softcap, int window, int q_heads, int kv_heads, int head_dim,
+                                              int32_t* status, gk_stream_t stream) {
+  return gk::prefill_entry(q, q_row_stride, pool_k, pool_v, slots, table, table_stride, table_entry_stride, page_tokens,
+                           table_rows, work, n_work, outs, n_outs, out_row_stride, gk::PrefillExtras{}, scale, softcap,
+                           window, q_heads, kv_heads, head_dim, status, stream);
+}
+
+extern "C" int gk_paged_prefill_tc_biased_multi_bf16(const void* q, int64_t q_row_stride, const void* pool_k,
+                                                     const void* pool_v, int64_t slots, const int32_t* table,
+                                                     int64_t table_stride, int64_t table_entry_stride, int page_tokens,
+                                                     const int32_t* table_rows, const int32_t* work, int64_t n_work,
+                                                     void* const* outs, int n_outs, int64_t out_row_stride,
+                                                     const float* slopes, const int32_t* row_limits, float scale,
+                                                     float softcap, int window, int q_heads, int kv_heads, int head_dim,
+                                                     int32_t* status, gk_stream_t stream) {
+  gk::PrefillExtras extras;
+  extras.slopes = slopes;
+  extras.row_limits = row_limits;
+  return gk::prefill_entry(q, q_row_stride, pool_k, pool_v, slots, table, table_stride, table_entry_stride, page_tokens,
+                           table_rows, work, n_work, outs, n_outs, out_row_stride, extras, scale, softcap, window, q_heads,
+                           kv_heads, head_dim, status, stream);
+}
+
+extern "C" int gk_shared_prefix_attn_bf16(const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v,
+                                          int64_t slots, const int32_t* table, int64_t table_stride,
+                                          int64_t table_entry_stride, int page_tokens, const int32_t* table_rows,
+                                          const int32_t* prefix_work, int64_t n_prefix_work, const int32_t* prefix_rows,
+                                          float* part_ml, float* part_o, const float* slopes, float scale, float softcap,
+                                          int window, int q_heads, int kv_heads, int head_dim, int32_t* status,
+                                          gk_stream_t stream) {
+  if (n_prefix_work == 0) return GK_OK;
+  if (!prefix_rows || q_heads <= 0 || kv_heads <= 0 || q_heads / kv_heads > GK_MAX_PACKED_ROWS)
+    return prefix_rows && q_heads > 0 && kv_heads > 0 ? GK_ERR_UNSUPPORTED : GK_ERR_INVALID_ARGUMENT;
+  gk::PrefillExtras extras;
+  extras.slopes = slopes;
+  extras.list = prefix_rows;
+  extras.part_ml = part_ml;
+  extras.part_o = part_o;
+  return gk::prefill_entry(q, q_row_stride, pool_k, pool_v, slots, table, table_stride, table_entry_stride, page_tokens,
+                           table_rows, prefix_work, n_prefix_work, nullptr, 0, 8, extras, scale, softcap, window, q_heads,
+                           kv_heads, head_dim, status, stream);
 }
 
 extern "C" int gk_paged_prefill_tc_bf16(const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v,

@@ -29,7 +29,8 @@ int64_t paged_attn_kv_tile(int64_t) { return GK_REFERENCE_KV_TILE; }
 at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tensor>& key_in,
                            const c10::optional<at::Tensor>& value_in, at::Tensor& key_pool, at::Tensor& value_pool,
                            const at::Tensor& locations, const at::Tensor& plan_tensor, int64_t head_dim, double scale,
-                           double softcap, int64_t sliding_window, const std::vector<at::Tensor>& pushed) {
+                           double softcap, int64_t sliding_window, const std::vector<at::Tensor>& pushed,
+                           const c10::optional<at::Tensor>& slopes_in = c10::nullopt) {
   const bool store = key_in.has_value() && key_in->defined();
   TORCH_CHECK(store == (value_in.has_value() && value_in->defined()),
               "GaudiRT attention: Q/K/V must be BF16 device matrices with matching rows");
@@ -65,6 +66,13 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
   TORCH_CHECK(key_pool.storage().unsafeGetStorageImpl() == value_pool.storage().unsafeGetStorageImpl() &&
                   value_address == key_address + half_bytes && key_address % 16 == 0,
               "GaudiRT attention: KV pool descriptor is not backed by combined storage");
+  const float* slopes = nullptr;
+  if (slopes_in.has_value() && slopes_in->defined()) {
+    TORCH_CHECK(slopes_in->is_cuda() && slopes_in->device() == device && slopes_in->scalar_type() == at::kFloat &&
+                    slopes_in->dim() == 1 && slopes_in->numel() == plan.query_heads && slopes_in->is_contiguous(),
+                "GaudiRT attention: slopes must be one contiguous FP32 device value per query head");
+    slopes = slopes_in->data_ptr<float>();
+  }
   // Row-strided column slices are read in place; anything else is packed first.
   const at::Tensor q = query.stride(1) == 1 ? query : query.contiguous();
   const at::Tensor k = !store || key.stride(1) == 1 ? key : key.contiguous();
@@ -103,7 +111,28 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
                                              locations.data_ptr<int32_t>(), plan.rows, key_pool.data_ptr(),
                                              value_pool.data_ptr(), plan.slots, (int)plan.kv_heads, (int)head_dim, status, s),
                  "KV store");
-  if (fused_store)
+  if (plan.n_prefix > 0)
+    // The keys that several sequences share, once for all of their rows; the states it leaves are merged by the
+    // attention kernel behind it.  It reads no row of this step, so the store may come after it.
+    check_status(gk_shared_prefix_attn_bf16(q.data_ptr(), q.stride(0), key_pool.data_ptr(), value_pool.data_ptr(), plan.slots,
+                                            plan.table.data_ptr<int32_t>(), plan.table_stride, plan.entry_stride,
+                                            plan.page_tokens, table_rows, words + plan.prefix_offset, plan.n_prefix,
+                                            words + plan.prefix_rows_offset, plan.part_ml.data_ptr<float>(),
+                                            plan.part_o.data_ptr<float>(), slopes, scale_f, softcap_f, (int)sliding_window,
+                                            (int)plan.query_heads, (int)plan.kv_heads, (int)head_dim, status, s),
+                 "shared prefix attention");
+  const int32_t* row_limits = plan.row_limits_offset >= 0 ? words + plan.row_limits_offset : nullptr;
+  if (slopes || row_limits || plan.n_prefix > 0)
+    check_status(gk_paged_attn_extended_multi_bf16(
+                     q.data_ptr(), q.stride(0), fused_store ? k.data_ptr() : nullptr, fused_store ? v.data_ptr() : nullptr,
+                     k.stride(0), v.stride(0), fused_store ? locations.data_ptr<int32_t>() : nullptr, key_pool.data_ptr(),
+                     value_pool.data_ptr(), plan.slots, plan.table.data_ptr<int32_t>(), plan.table_stride,
+                     plan.entry_stride, plan.page_tokens, table_rows, words, plan.n_work, outs.data(), (int)outs.size(),
+                     out_stride, plan.part_ml.data_ptr<float>(), plan.part_o.data_ptr<float>(), counters, slopes, row_limits,
+                     plan.n_prefix > 0 ? words + plan.parts_before_offset : nullptr, scale_f, softcap_f,
+                     (int)sliding_window, (int)plan.query_heads, (int)plan.kv_heads, (int)head_dim, status, s),
+                 "paged attention");
+  else if (fused_store)
     check_status(gk_paged_attn_store_multi_bf16(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), k.stride(0),
                                                 v.stride(0), locations.data_ptr<int32_t>(), key_pool.data_ptr(),
                                                 value_pool.data_ptr(), plan.slots, plan.table.data_ptr<int32_t>(),
@@ -129,12 +158,18 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
   if (plan.n_prefill > 0)
     // Query tiles of multi-row sequences: tcgen05 kernel, same destinations (a mixed prefill + decode
     // step is one call, as in src/bridge/paged_attention.cpp:251-345; the two kernels write disjoint rows).
-    check_status(gk_paged_prefill_tc_multi_bf16(q.data_ptr(), q.stride(0), key_pool.data_ptr(), value_pool.data_ptr(),
-                                                plan.slots, plan.table.data_ptr<int32_t>(), plan.table_stride,
-                                                plan.entry_stride, plan.page_tokens,
-                                                table_rows, words + plan.prefill_offset, plan.n_prefill, outs.data(), (int)outs.size(),
-                                                out_stride, scale_f, softcap_f, (int)sliding_window, (int)plan.query_heads,
-                                                (int)plan.kv_heads, (int)head_dim, status, s),
+    check_status(slopes || row_limits
+                     ? gk_paged_prefill_tc_biased_multi_bf16(
+                           q.data_ptr(), q.stride(0), key_pool.data_ptr(), value_pool.data_ptr(), plan.slots,
+                           plan.table.data_ptr<int32_t>(), plan.table_stride, plan.entry_stride, plan.page_tokens, table_rows,
+                           words + plan.prefill_offset, plan.n_prefill, outs.data(), (int)outs.size(), out_stride, slopes,
+                           row_limits, scale_f, softcap_f, (int)sliding_window, (int)plan.query_heads, (int)plan.kv_heads,
+                           (int)head_dim, status, s)
+                     : gk_paged_prefill_tc_multi_bf16(
+                           q.data_ptr(), q.stride(0), key_pool.data_ptr(), value_pool.data_ptr(), plan.slots,
+                           plan.table.data_ptr<int32_t>(), plan.table_stride, plan.entry_stride, plan.page_tokens, table_rows,
+                           words + plan.prefill_offset, plan.n_prefill, outs.data(), (int)outs.size(), out_stride, scale_f,
+                           softcap_f, (int)sliding_window, (int)plan.query_heads, (int)plan.kv_heads, (int)head_dim, status, s),
                  "tensor-core prefill");
   return output;
 }
@@ -154,10 +189,11 @@ at::Tensor paged_attn_validated(const at::Tensor& query, const at::Tensor& key, 
 void paged_attn_push(const at::Tensor& query, const c10::optional<at::Tensor>& key,
                      const c10::optional<at::Tensor>& value, at::Tensor& key_pool,
                      at::Tensor& value_pool, const at::Tensor& locations, const at::Tensor& plan_tensor,
-                     at::TensorList outputs, int64_t head_dim, double scale, double softcap, int64_t sliding_window) {
+                     at::TensorList outputs, int64_t head_dim, double scale, double softcap, int64_t sliding_window,
+                     const c10::optional<at::Tensor>& slopes) {
   TORCH_CHECK(!outputs.empty(), "GaudiRT attention: gather destinations are required");
   paged_attn_impl(query, key, value, key_pool, value_pool, locations, plan_tensor, head_dim, scale, softcap,
-                  sliding_window, outputs.vec());
+                  sliding_window, outputs.vec(), slopes);
 }
 
 // Completion barrier after the pushes: flags[p] aliases rank p's int32[world] flag array.
@@ -382,6 +418,25 @@ at::Tensor paged_attn_stored(const at::Tensor& query, at::Tensor& key_pool, at::
                          head_dim, scale, softcap, sliding_window, {});
 }
 
+// paged_attn with a bias that falls with the distance between row and key: the capped score of key j for a row at
+// position p of query head h gets -slopes[h] * |p - j|.  Without key / value the step's rows are in the pool already.
+// Not part of the reference surface.
+at::Tensor paged_attn_biased(const at::Tensor& query, const c10::optional<at::Tensor>& key,
+                             const c10::optional<at::Tensor>& value, at::Tensor& key_pool, at::Tensor& value_pool,
+                             const c10::intrusive_ptr<PagedMetadata>& metadata, const at::Tensor& slopes, int64_t head_dim,
+                             double scale, double softcap, int64_t sliding_window) {
+  TORCH_CHECK(metadata, "GaudiRT paged attention: metadata is required");
+  TORCH_CHECK(query.dim() == 2 && key_pool.dim() == 3 && (head_dim == 64 || head_dim == 128 || head_dim == 256),
+              "GaudiRT paged attention: invalid tensor ranks or head dimension");
+  TORCH_CHECK(slopes.defined(), "GaudiRT attention: slopes must be one contiguous FP32 device value per query head");
+  const auto q_heads = query.size(1) / head_dim;
+  const auto kv_heads = key_pool.size(1);
+  auto plan = sliding_window > 0 ? metadata->attention_plan_for(q_heads, kv_heads, head_dim, sliding_window)
+                                 : metadata->attention_plan(q_heads, kv_heads, head_dim);
+  return paged_attn_impl(query, key, value, key_pool, value_pool, metadata->row_locations(), plan, head_dim, scale, softcap,
+                         sliding_window, {}, slopes);
+}
+
 void set_fused_kv_store(bool on) { fuse_kv_store_flag().store(on); }
 
 // Reads and clears the device status word of the current device (synchronises the stream).
@@ -419,6 +474,10 @@ TORCH_LIBRARY(gaudirt, m) {
       .def("last_token_indices", &PagedMetadata::last_token_indices)
       .def("token_ids", &PagedMetadata::token_ids)
       .def("vocabulary", &PagedMetadata::vocabulary)
+      .def("_share_prefixes_", &PagedMetadata::share_prefixes_)
+      .def("_set_prefix_mask_", &PagedMetadata::set_prefix_mask_)
+      .def("_set_prefix_sharing", &PagedMetadata::set_prefix_sharing)
+      .def("_last_plan_prefix_records", &PagedMetadata::last_plan_prefix_records)
       .def("_set_split_tokens", &PagedMetadata::set_split_tokens)
       .def("_set_prefill_min_rows", &PagedMetadata::set_prefill_min_rows)
       .def("_set_fused_combine", &PagedMetadata::set_fused_combine)
@@ -431,7 +490,10 @@ TORCH_LIBRARY(gaudirt, m) {
         "int head_dim, float scale, float softcap=0.0, int sliding_window=-1) -> Tensor");
   m.def("_paged_attn_push(Tensor query, Tensor? key, Tensor? value, Tensor(a!) key_pool, Tensor(b!) value_pool, "
         "Tensor locations, Tensor plan, Tensor(c!)[] outputs, int head_dim, float scale, float softcap=0.0, "
-        "int sliding_window=-1) -> ()");
+        "int sliding_window=-1, Tensor? slopes=None) -> ()");
+  m.def("_paged_attn_biased(Tensor query, Tensor? key, Tensor? value, Tensor(a!) key_pool, Tensor(b!) value_pool, "
+        "__torch__.torch.classes.gaudirt.PagedMetadata metadata, Tensor slopes, int head_dim, float scale, "
+        "float softcap=0.0, int sliding_window=-1) -> Tensor");
   m.def("_paged_attn_stored(Tensor query, Tensor(a!) key_pool, Tensor(b!) value_pool, "
         "__torch__.torch.classes.gaudirt.PagedMetadata metadata, int head_dim, float scale, "
         "float softcap=0.0, int sliding_window=-1) -> Tensor");
@@ -455,6 +517,9 @@ TORCH_LIBRARY(gaudirt, m) {
   m.def("_take_device_status() -> int", &gaudirt_b200::take_device_status);
   m.def("_allocate_paged_slots", &gaudirt_b200::allocate_paged_slots);
   m.def("_allocate_paged_slots_into", &gaudirt_b200::allocate_paged_slots_into);
+  m.def("_extend_paged_requests(Tensor(a!) mapping, Tensor batch_requests, Tensor lengths, Tensor new_tokens, "
+        "Tensor free_pages, Tensor used_pages, int page_size, int rows) -> "
+        "(Tensor locations, Tensor positions, Tensor row_requests, Tensor row_offsets, Tensor next_lengths, Tensor next_used)");
   m.def("_release_paged_slots", &gaudirt_b200::release_paged_slots);
   m.def("_advance_decode_lengths(Tensor seq_lens, Tensor orig_seq_lens) -> (Tensor, Tensor)");
   m.def("sample_from_logits(Tensor logits, Tensor temperatures, Tensor top_ps, Tensor top_ks, Tensor min_ps, "
@@ -473,6 +538,7 @@ TORCH_LIBRARY_IMPL(gaudirt, CUDA, m) {
   m.impl("paged_attn", TORCH_FN(gaudirt_b200::paged_attn));
   m.impl("_paged_attn_validated", TORCH_FN(gaudirt_b200::paged_attn_validated));
   m.impl("_paged_attn_push", TORCH_FN(gaudirt_b200::paged_attn_push));
+  m.impl("_paged_attn_biased", TORCH_FN(gaudirt_b200::paged_attn_biased));
   m.impl("_paged_attn_stored", TORCH_FN(gaudirt_b200::paged_attn_stored));
   m.impl("_rotary_kv_store", TORCH_FN(gaudirt_b200::rotary_kv_store));
   m.impl("_peer_barrier", TORCH_FN(gaudirt_b200::peer_barrier));
@@ -482,6 +548,7 @@ TORCH_LIBRARY_IMPL(gaudirt, CUDA, m) {
   m.impl("rotary_embedding", TORCH_FN(gaudirt_b200::rotary_embedding));
   m.impl("rotary_embedding_positions", TORCH_FN(gaudirt_b200::rotary_embedding_positions));
   m.impl("_rotary_embedding_validated", TORCH_FN(gaudirt_b200::rotary_embedding_validated));
+  m.impl("_extend_paged_requests", TORCH_FN(gaudirt_b200::extend_paged_requests));
   m.impl("_advance_decode_lengths", TORCH_FN(gaudirt_b200::advance_decode_lengths));
   m.impl("sample_from_logits", TORCH_FN(gaudirt_b200::sample_from_logits));
   m.impl("apply_token_bitmask_inplace_", TORCH_FN(gaudirt_b200::apply_token_bitmask_inplace_));

@@ -11,6 +11,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <cmath>
 #include <cstring>
@@ -76,6 +77,9 @@ struct AttentionPlan {
   int64_t rows = 0, slots = 0, query_heads = 0, kv_heads = 0, head_dim = 0, sliding_window = -1;
   int64_t n_work = 0, n_combine = 0, combine_offset = 0, table_stride = 0, entry_stride = 1;
   int64_t n_prefill = 0, prefill_offset = 0;   // query tiles for the tensor-core prefill kernel
+  int64_t n_prefix = 0, prefix_offset = 0;     // shared prefixes: records, listed rows, and per row the states in front
+  int64_t prefix_rows_offset = 0, parts_before_offset = 0;
+  int64_t row_limits_offset = -1;              // last key each row sees (two-way prefixes only)
   int page_tokens = 1;
   // Every sequence of the step is one query block of the decode kernel (no other CTA reads a new row):
   // the KV store may then ride in the attention launch.
@@ -230,6 +234,7 @@ class PagedMetadata : public torch::CustomClassHolder {
     // writes, so its sequences never read each other's new rows; the scheduler-owned form skips
     // that check and nothing is known here.
     rows_independent_ = !scheduler_owned;
+    scheduler_owned_ = scheduler_owned;
     const auto i32 = at::TensorOptions().dtype(at::kInt).device(device);
     auto seq_device = staging.to(device, /*non_blocking=*/true);
     // Strided views (a column of a scheduler's packed buffer) are packed first, like the
@@ -379,6 +384,78 @@ class PagedMetadata : public torch::CustomClassHolder {
                      device_status(device.index()).data_ptr<int32_t>(),
                      stream_of(at::cuda::getCurrentCUDAStream(device.index()))),
                  "device metadata");
+    check_shared_tables();
+  }
+
+  // Declares which sequences of the step begin with the same cached tokens in the same slots: sequence i is in group
+  // `groups[i]` (-1 = none), and the first `prefix_tokens[g]` positions of every member of group g hold the same slots.
+  // Plans built afterwards attend to such a prefix once for all rows of the group (where that pays); every attention
+  // operator over this metadata then computes what it computed before.  Every member's new rows lie behind the prefix.
+  // The table rows are compared on the device and a difference is refused here (in `_revalidate_`: GK_DEV_BAD_METADATA
+  // in the status word); a table owned by the scheduler is vouched for by it.  Not part of the reference surface.
+  void share_prefixes_(std::vector<int64_t> groups, std::vector<int64_t> prefix_tokens) {
+    const int64_t n_seq = static_cast<int64_t>(sequences_.size() / 4);
+    TORCH_CHECK(plans_.empty(), "GaudiRT shared prefix: the metadata is already bound to an attention plan");
+    TORCH_CHECK(static_cast<int64_t>(groups.size()) == n_seq, "GaudiRT shared prefix: expected one group per sequence");
+    std::vector<int32_t> group_of(static_cast<size_t>(n_seq)), tokens, pairs;
+    for (const int64_t t : prefix_tokens) {
+      TORCH_CHECK(t >= 0 && t <= INT32_MAX, "GaudiRT shared prefix: invalid prefix length");
+      tokens.push_back(static_cast<int32_t>(t));
+    }
+    std::vector<int64_t> first(prefix_tokens.size(), -1);
+    for (int64_t i = 0; i < n_seq; ++i) {
+      const int64_t g = groups[static_cast<size_t>(i)];
+      TORCH_CHECK(g >= -1 && g < static_cast<int64_t>(tokens.size()), "GaudiRT shared prefix: group out of range");
+      group_of[static_cast<size_t>(i)] = static_cast<int32_t>(g);
+      if (g < 0) continue;
+      const int32_t* seq = &sequences_[static_cast<size_t>(i) * 4];
+      TORCH_CHECK(tokens[g] <= context_, "GaudiRT shared prefix: invalid prefix length");
+      TORCH_CHECK(seq[2] >= tokens[g], "GaudiRT shared prefix: sequence ", i, " begins inside the prefix of its group");
+      if (first[g] < 0) {
+        first[g] = i;
+      } else if (tokens[g] > 0) {
+        pairs.insert(pairs.end(), {sequences_[static_cast<size_t>(first[g]) * 4 + 3], seq[3], tokens[g], static_cast<int32_t>(i)});
+      }
+    }
+    if (!scheduler_owned_ && !pairs.empty()) {
+      const auto device = locations_.device();
+      c10::cuda::CUDAGuard guard(device);
+      auto staging = at::empty({static_cast<int64_t>(pairs.size())}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
+      std::memcpy(staging.data_ptr<int32_t>(), pairs.data(), pairs.size() * sizeof(int32_t));
+      shared_pairs_ = staging.to(device, /*non_blocking=*/true);
+      shared_verdict_ = at::empty({1}, at::TensorOptions().dtype(at::kInt).device(device));
+      check_shared_tables();
+      const int32_t bad = shared_verdict_.item<int32_t>();
+      if (bad != -1) {
+        clear_status_bits(device.index(), GK_DEV_BAD_METADATA);
+        shared_pairs_ = at::Tensor();
+        TORCH_CHECK(false, "GaudiRT shared prefix: sequence ", bad, " does not hold the slots of its group's prefix");
+      }
+    } else {
+      shared_pairs_ = at::Tensor();
+    }
+    shared_groups_ = std::move(group_of);
+    shared_tokens_ = std::move(tokens);
+  }
+
+  // Two-way prefixes (prefix-LM masks): the rows of sequence i see every key below prefix_tokens[i], also those behind
+  // them, besides the causal ones; 0 = causal.  The prefix ends at or before the sequence's last row, so that all of
+  // its keys are in the pool when the step attends.  Not part of the reference surface.
+  void set_prefix_mask_(std::vector<int64_t> prefix_tokens) {
+    TORCH_CHECK(plans_.empty(), "GaudiRT prefix mask: the metadata is already bound to an attention plan");
+    const int64_t n_seq = static_cast<int64_t>(sequences_.size() / 4);
+    TORCH_CHECK(static_cast<int64_t>(prefix_tokens.size()) == n_seq, "GaudiRT prefix mask: expected one prefix per sequence");
+    std::vector<int32_t> two_way;
+    bool any = false;
+    for (int64_t i = 0; i < n_seq; ++i) {
+      const int32_t* seq = &sequences_[static_cast<size_t>(i) * 4];
+      const int64_t t = prefix_tokens[static_cast<size_t>(i)];
+      TORCH_CHECK(t >= 0 && t <= static_cast<int64_t>(seq[2]) + seq[1],
+                  "GaudiRT prefix mask: the prefix of sequence ", i, " reaches past its last row");
+      any = any || t > seq[2] + 1;                     // a row can only see more than its causal keys below that
+      two_way.push_back(static_cast<int32_t>(t));
+    }
+    two_way_ = any ? std::move(two_way) : std::vector<int32_t>();
   }
 
   int64_t rows() const { return rows_; }
@@ -425,34 +502,85 @@ class PagedMetadata : public torch::CustomClassHolder {
     const int64_t n_seq = static_cast<int64_t>(sequences_.size() / 4);
     const int window = static_cast<int>(sliding_window);
     // Multi-row sequences go to the tensor-core prefill kernel, the rest -- decode rows and very
-    // short chunks -- to the split-KV decode kernel.
-    int64_t n_prefill = 0, n_rest = n_seq;
-    std::vector<int32_t> rest(sequences_);
-    const bool tensor_core = prefill_min_rows_ >= 0;
-    if (tensor_core)
-      check_status(gk_prefill_plan_build(sequences_.data(), n_seq, (int)query_heads, (int)kv_heads, window,
-                                         prefill_min_rows_, nullptr, 0, &n_prefill, rest.data(), &n_rest),
-                   "prefill plan");
-    int64_t n_work = 0, n_combine = 0, entries = 0;
-    if (n_rest > 0)
-      check_status(gk_attention_plan_build(rest.data(), n_rest, (int)query_heads, (int)kv_heads, (int)head_dim, window,
-                                           sm_count, split_tokens_, nullptr, 0, &n_work, nullptr, 0, &n_combine, &entries),
-                   "attention plan");
+    // short chunks -- to the split-KV decode kernel.  Short chunks of a group that is attended to together stay with
+    // its decode rows; a longer one reads the prefix once per 256 packed rows as it is and takes no part in the group.
+    const int64_t min_saved = prefix_sharing_ > 0 ? 0 : kSharedPrefixMinSavedBytes;
+    const std::vector<char> together = short_group_members(query_heads, kv_heads, head_dim, min_saved);
+    std::vector<int32_t> offered, offered_two_way, rest;
+    for (int64_t i = 0; i < n_seq; ++i) {
+      const int32_t* seq = &sequences_[static_cast<size_t>(i) * 4];
+      if (prefill_min_rows_ < 0 || (!together.empty() && together[static_cast<size_t>(i)])) {
+        rest.insert(rest.end(), seq, seq + 4);
+      } else {
+        offered.insert(offered.end(), seq, seq + 4);
+        if (!two_way_.empty()) offered_two_way.push_back(two_way_[static_cast<size_t>(i)]);
+      }
+    }
+    const int64_t n_offered = static_cast<int64_t>(offered.size() / 4);
+    int64_t n_prefill = 0, n_left = 0;
+    std::vector<int32_t> left(offered.size());
+    auto build_prefill = [&](int32_t* work) {
+      return gk_prefill_plan_build_two_way(offered.data(), n_offered, two_way_.empty() ? nullptr : offered_two_way.data(),
+                                           (int)query_heads, (int)kv_heads, window, prefill_min_rows_, work, n_prefill,
+                                           &n_prefill, left.data(), &n_left);
+    };
+    if (n_offered > 0) check_status(build_prefill(nullptr), "prefill plan");
+    rest.insert(rest.end(), left.begin(), left.begin() + n_left * 4);
+    const int64_t n_rest = static_cast<int64_t>(rest.size() / 4);
+    // back into row order, and what was declared per sequence carried over
+    {
+      std::vector<std::array<int32_t, 4>> ordered(static_cast<size_t>(n_rest));
+      std::memcpy(ordered.data(), rest.data(), rest.size() * sizeof(int32_t));
+      std::sort(ordered.begin(), ordered.end());
+      std::memcpy(rest.data(), ordered.data(), rest.size() * sizeof(int32_t));
+    }
+    std::vector<int32_t> rest_groups, rest_two_way;
+    for (int64_t i = 0, at = 0; i < n_seq && at < n_rest; ++i) {
+      if (sequences_[static_cast<size_t>(i) * 4] != rest[static_cast<size_t>(at) * 4]) continue;
+      rest_groups.push_back(shared_groups_.empty() || prefix_sharing_ == 0 ? -1 : shared_groups_[static_cast<size_t>(i)]);
+      rest_two_way.push_back(two_way_.empty() ? 0 : two_way_[static_cast<size_t>(i)]);
+      ++at;
+    }
+    const int64_t n_groups = static_cast<int64_t>(shared_tokens_.size());
+    int64_t n_work = 0, n_combine = 0, entries = 0, n_prefix = 0, n_prefix_rows = 0;
+    auto build = [&](int32_t* work, int32_t* combine, int32_t* prefix_work, int32_t* prefix_rows) {
+      return gk_shared_prefix_plan_build(rest.data(), n_rest, rest_two_way.data(), rest_groups.data(), shared_tokens_.data(),
+                                         n_groups, (int)query_heads, (int)kv_heads, (int)head_dim, window, sm_count,
+                                         split_tokens_, prefix_split_tokens_, min_saved, work, n_work, &n_work, combine,
+                                         n_combine, &n_combine, &entries, prefix_work, n_prefix, &n_prefix, prefix_rows,
+                                         n_prefix_rows, &n_prefix_rows);
+    };
+    if (n_rest > 0) check_status(build(nullptr, nullptr, nullptr, nullptr), "attention plan");
     const int64_t combine_offset = n_work * GK_WORK_WORDS;
     const int64_t prefill_offset = combine_offset + n_combine * GK_COMBINE_WORDS;
-    const int64_t words = std::max<int64_t>(4, prefill_offset + n_prefill * GK_WORK_WORDS);
+    const int64_t prefix_offset = prefill_offset + n_prefill * GK_WORK_WORDS;
+    const int64_t prefix_rows_offset = prefix_offset + n_prefix * GK_WORK_WORDS;
+    const int64_t parts_before_offset = prefix_rows_offset + n_prefix_rows * 4;
+    const int64_t row_limits_offset = parts_before_offset + (n_prefix > 0 ? rows_ : 0);
+    const int64_t words = std::max<int64_t>(4, row_limits_offset + (two_way_.empty() ? 0 : rows_));
     auto staging = at::empty({words}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
     int32_t* host = staging.data_ptr<int32_t>();
     if (n_rest > 0)
-      check_status(gk_attention_plan_build(rest.data(), n_rest, (int)query_heads, (int)kv_heads, (int)head_dim, window,
-                                           sm_count, split_tokens_, host, n_work, &n_work, host + combine_offset,
-                                           n_combine, &n_combine, &entries),
-                   "attention plan");
-    if (n_prefill > 0)
-      check_status(gk_prefill_plan_build(sequences_.data(), n_seq, (int)query_heads, (int)kv_heads, window,
-                                         prefill_min_rows_, host + prefill_offset, n_prefill, &n_prefill, rest.data(),
-                                         &n_rest),
-                   "prefill plan");
+      check_status(build(host, host + combine_offset, host + prefix_offset, host + prefix_rows_offset), "attention plan");
+    if (n_prefill > 0) check_status(build_prefill(host + prefill_offset), "prefill plan");
+    if (n_prefix > 0) {
+      int32_t* before = host + parts_before_offset;
+      std::fill(before, before + rows_, 0);
+      for (int64_t i = 0; i < n_prefix; ++i) {               // parts of a row: one more than its highest part index
+        const int32_t* w = host + prefix_offset + i * GK_WORK_WORDS;
+        for (int32_t r = 0; r < w[1]; ++r) {
+          int32_t& parts = before[host[prefix_rows_offset + ((int64_t)w[0] + r) * 4]];
+          parts = std::max(parts, w[2] + 1);
+        }
+      }
+    }
+    if (!two_way_.empty()) {
+      int32_t* limit = host + row_limits_offset;
+      for (int64_t i = 0; i < n_seq; ++i)
+        for (int32_t r = 0; r < sequences_[static_cast<size_t>(i) * 4 + 1]; ++r)
+          limit[sequences_[static_cast<size_t>(i) * 4] + r] =
+              std::max(sequences_[static_cast<size_t>(i) * 4 + 2] + r, two_way_[static_cast<size_t>(i)] - 1);
+    }
     auto plan = std::make_unique<AttentionPlan>();
     plan->buffer = staging.to(device, /*non_blocking=*/true);
     const auto f32 = at::TensorOptions().dtype(at::kFloat).device(device);
@@ -466,7 +594,8 @@ class PagedMetadata : public torch::CustomClassHolder {
     // that the fused form costs nothing even with hundreds of them, and it saves the launch.
     int32_t most_splits = 0;
     for (int64_t i = 0; i < n_combine; ++i) most_splits = std::max(most_splits, host[combine_offset + i * GK_COMBINE_WORDS + 3]);
-    const bool fuse = fused_combine_ > 0 || (fused_combine_ < 0 && (n_combine * 5 <= sm_count * 2 || most_splits <= 2));
+    // Behind a shared prefix the merge is always part of the attention kernel: its splits follow the prefix's states.
+    const bool fuse = n_prefix > 0 || fused_combine_ > 0 || (fused_combine_ < 0 && (n_combine * 5 <= sm_count * 2 || most_splits <= 2));
     last_plan_fused_ = n_combine > 0 && fuse;
     if (n_combine > 0 && fuse)
       plan->counters = at::zeros({rows_ * kv_heads}, at::TensorOptions().dtype(at::kInt).device(device));
@@ -488,6 +617,12 @@ class PagedMetadata : public torch::CustomClassHolder {
     plan->combine_offset = combine_offset;
     plan->n_prefill = n_prefill;
     plan->prefill_offset = prefill_offset;
+    plan->n_prefix = n_prefix;
+    plan->prefix_offset = prefix_offset;
+    plan->prefix_rows_offset = prefix_rows_offset;
+    plan->parts_before_offset = parts_before_offset;
+    plan->row_limits_offset = two_way_.empty() ? -1 : row_limits_offset;
+    last_plan_prefix_records_ = n_prefix;
     {
       const int64_t block_rows = std::max<int64_t>(1, GK_MAX_PACKED_ROWS / (query_heads / kv_heads));
       bool single = n_prefill == 0 && n_work > 0 && rows_independent_;
@@ -519,6 +654,16 @@ class PagedMetadata : public torch::CustomClassHolder {
     prefill_min_rows_ = static_cast<int>(rows);
   }
 
+  // Whether declared prefixes are attended to together: -1 = where it pays, 0 = never, 1 = always; and the longest piece
+  // of a prefix one CTA takes (0 = chosen from the SM count).  Test and tuning hook.
+  void set_prefix_sharing(int64_t mode, int64_t split_tokens) {
+    TORCH_CHECK(mode >= -1 && mode <= 1 && split_tokens >= 0 && split_tokens <= INT32_MAX,
+                "GaudiRT shared prefix: invalid sharing mode");
+    prefix_sharing_ = static_cast<int>(mode);
+    prefix_split_tokens_ = static_cast<int>(split_tokens);
+  }
+  int64_t last_plan_prefix_records() const { return last_plan_prefix_records_; }
+
   int64_t rows_ = 0, slots_ = 0, request_count_ = 0, context_ = 0, vocabulary_ = 0, page_tokens_ = 1;
   // -1: decide from the schedule, 0: separate combine kernel, 1: combine fused into attention.
   bool last_plan_fuses_combine() const { return last_plan_fused_; }
@@ -528,6 +673,45 @@ class PagedMetadata : public torch::CustomClassHolder {
   }
   int split_tokens_ = 0, prefill_min_rows_ = 0, fused_combine_ = -1;
   bool last_plan_fused_ = false;       // whether the plan built last merges its splits inside the attention kernel
+  // Reading less than this again costs less than one more launch and the merge of the prefix's states.
+  static constexpr int64_t kSharedPrefixMinSavedBytes = int64_t{24} << 20;
+  int prefix_sharing_ = -1, prefix_split_tokens_ = 0;
+  int64_t last_plan_prefix_records_ = 0;
+  std::vector<int32_t> shared_groups_, shared_tokens_, two_way_;   // per sequence, per group, per sequence
+  at::Tensor shared_pairs_, shared_verdict_;                       // table rows that must agree, and the first that does not
+  bool scheduler_owned_ = false;
+  // Sequences of at most kSharedPackedRows packed rows whose groups are worth attending to together.
+  static constexpr int64_t kSharedPackedRows = 64;
+  std::vector<char> short_group_members(int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t min_saved) const {
+    if (shared_groups_.empty() || prefix_sharing_ == 0) return {};
+    std::vector<char> in(shared_groups_.size(), 0);
+    std::vector<int64_t> members(shared_tokens_.size(), 0);
+    for (size_t i = 0; i < in.size(); ++i) {
+      if (shared_groups_[i] < 0 || sequences_[i * 4 + 1] * (query_heads / kv_heads) > kSharedPackedRows) continue;
+      in[i] = 1;
+      ++members[static_cast<size_t>(shared_groups_[i])];
+    }
+    for (size_t i = 0; i < in.size(); ++i)
+      if (in[i]) {
+        const int64_t count = members[static_cast<size_t>(shared_groups_[i])], tokens = shared_tokens_[static_cast<size_t>(shared_groups_[i])];
+        in[i] = count >= 2 && tokens > 0 && (count - 1) * tokens * kv_heads * head_dim * 4 >= min_saved;
+      }
+    return in;
+  }
+  // Compares the table rows of every group on the device; launches only.
+  void check_shared_tables() {
+    if (!shared_pairs_.defined()) return;
+    const auto device = locations_.device();
+    c10::cuda::CUDAGuard guard(device);
+    check_status(gk_shared_prefix_check(mapping_.data_ptr<int32_t>(), mapping_.size(0), mapping_.size(1), mapping_.stride(0),
+                                        batch_requests_.defined() ? batch_requests_.data_ptr<int32_t>() : nullptr,
+                                        batch_requests_.defined() ? batch_requests_.numel() : mapping_.size(0),
+                                        shared_pairs_.data_ptr<int32_t>(), shared_pairs_.numel() / 4,
+                                        shared_verdict_.data_ptr<int32_t>(),
+                                        device_status(device.index()).data_ptr<int32_t>(),
+                                        stream_of(at::cuda::getCurrentCUDAStream(device.index()))),
+                 "shared prefix");
+  }
   bool rows_independent_ = false;   // no sequence of the step reads a row that another sequence writes
   at::Tensor locations_, requests_, positions_, mapping_, header_, batch_requests_, token_ids_, last_token_indices_;
   at::Tensor dev_seq_, dev_workspace_, dev_verdict_, dev_row_status_;   // device-validated forms only (revalidate_)
@@ -543,6 +727,9 @@ std::tuple<at::Tensor, int64_t> allocate_paged_slots(const at::Tensor& last_slot
 std::tuple<at::Tensor, at::Tensor, int64_t> allocate_paged_slots_into(
     const at::Tensor& last_slots, const at::Tensor& free_pages, std::vector<int64_t> prefixes,
     std::vector<int64_t> lengths, int64_t page_size, at::Tensor& mapping, const at::Tensor& batch_requests);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> extend_paged_requests(
+    at::Tensor& mapping, const at::Tensor& batch_requests, const at::Tensor& lengths, const at::Tensor& new_tokens,
+    const at::Tensor& free_pages, const at::Tensor& used_pages, int64_t page_size, int64_t rows);
 at::Tensor release_paged_slots(const at::Tensor& slots, int64_t page_size, int64_t max_pages);
 std::tuple<at::Tensor, at::Tensor> advance_decode_lengths(const at::Tensor& seq_lens, const at::Tensor& orig_seq_lens);
 at::Tensor oproj(const at::Tensor& input, const at::Tensor& weight);

@@ -80,6 +80,53 @@ std::tuple<at::Tensor, at::Tensor, int64_t> allocate_paged_slots_into(
   return {result, locations, pages};
 }
 
+// The slot list, the table rows and the index vectors of a step from lengths that live on the device: what
+// `_allocate_paged_slots_into` does from host lists, without a host list or a read-back.  Rows past the last new token
+// hold -1.  A batch that cannot be served whole (a request out of range or named twice, a length that leaves the table,
+// more new tokens than `rows`, too few free pages) changes nothing, blanks every row and sets GK_DEV_BAD_METADATA.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> extend_paged_requests(
+    at::Tensor& mapping, const at::Tensor& batch_requests, const at::Tensor& lengths, const at::Tensor& new_tokens,
+    const at::Tensor& free_pages, const at::Tensor& used_pages, int64_t page_size, int64_t rows) {
+  require_indices(lengths);
+  require_indices(free_pages);
+  require_indices(used_pages);
+  const auto device = lengths.device();
+  TORCH_CHECK(mapping.is_cuda() && mapping.device() == device && mapping.scalar_type() == at::kInt && mapping.dim() == 2 &&
+                  mapping.size(0) > 0 && mapping.size(1) > 0 && mapping.size(1) <= INT32_MAX && mapping.stride(1) == 1 &&
+                  mapping.stride(0) >= mapping.size(1),
+              "GaudiRT paged allocator: expected an int32 request map with rows of its own on the same device");
+  for (const auto& t : {batch_requests, new_tokens})
+    TORCH_CHECK(t.is_cuda() && t.device() == device && t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() &&
+                    t.numel() == lengths.numel(),
+                "GaudiRT paged allocator: expected contiguous int32 request ids and token counts, one per length");
+  TORCH_CHECK(free_pages.device() == device && used_pages.device() == device && used_pages.numel() == 1,
+              "GaudiRT paged allocator: expected the free page list and its used count on the same device");
+  const int64_t batch = lengths.numel();
+  TORCH_CHECK(page_size >= 1 && page_size <= INT32_MAX && rows > 0 && rows <= (int64_t{1} << 30) && batch > 0 &&
+                  batch <= 65536 && mapping.size(0) <= 262144,
+              "GaudiRT paged allocator: unsupported page size, row count or request count");
+  c10::cuda::CUDAGuard guard(device);
+  const auto i32 = batch_requests.options(), i64 = lengths.options();
+  auto locations = at::empty({rows}, i32), positions = at::empty({rows}, i32), row_requests = at::empty({rows}, i32);
+  auto row_offsets = at::empty({batch + 1}, i32);
+  auto next_lengths = at::empty({batch}, i64), next_used = at::empty({1}, i64);
+  uint64_t bytes = 0;
+  check_status(gk_extend_requests_workspace_bytes(batch, &bytes), "paged allocator");
+  at::Tensor workspace;
+  if (bytes > 0) workspace = at::empty({static_cast<int64_t>(bytes)}, i32.dtype(at::kByte));
+  check_status(gk_extend_requests(mapping.data_ptr<int32_t>(), mapping.size(0), mapping.size(1), mapping.stride(0),
+                                  batch_requests.data_ptr<int32_t>(), lengths.data_ptr<int64_t>(),
+                                  new_tokens.data_ptr<int32_t>(), batch, free_pages.data_ptr<int64_t>(), free_pages.numel(),
+                                  used_pages.data_ptr<int64_t>(), page_size, rows,
+                                  workspace.defined() ? workspace.data_ptr() : nullptr, locations.data_ptr<int32_t>(),
+                                  positions.data_ptr<int32_t>(), row_requests.data_ptr<int32_t>(),
+                                  row_offsets.data_ptr<int32_t>(), next_lengths.data_ptr<int64_t>(),
+                                  next_used.data_ptr<int64_t>(), device_status(device.index()).data_ptr<int32_t>(),
+                                  stream_of(at::cuda::getCurrentCUDAStream(device.index()))),
+               "paged allocator");
+  return {locations, positions, row_requests, row_offsets, next_lengths, next_used};
+}
+
 at::Tensor release_paged_slots(const at::Tensor& slots, int64_t page_size, int64_t max_pages) {
   require_indices(slots);
   TORCH_CHECK(page_size >= 1 && page_size <= INT32_MAX && max_pages > 0 && max_pages <= INT32_MAX && slots.numel() > 0 &&

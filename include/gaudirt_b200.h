@@ -208,6 +208,84 @@ GK_API int gk_paged_prefill_tc_bf16(const void* q, int64_t q_row_stride, const v
                              int window, int q_heads, int kv_heads, int head_dim,
                              int32_t* status, gk_stream_t stream);
 
+/* ---- distance bias and two-way prefixes --------------------------------------------------------
+ * No counterpart in the reference.  The extended forms of gk_paged_attn_store_multi_bf16 (new_k, new_v
+ * and locations may all be NULL: no store) and gk_paged_prefill_tc_multi_bf16.  After scale and softcap
+ * the score of key j for a row at position p of query head h gets
+ *   s -= slopes[h] * |p - j|          slopes: fp32 [q_heads], finite; NULL = none
+ * and a row sees the keys j <= row_limits[row] instead of j <= p (int32 [rows], row_limits[row] >= the
+ * row's position, non-decreasing within a sequence; NULL = causal).  A sliding window still counts from
+ * the row's own position.  The plan must cover the keys: gk_shared_prefix_plan_build and
+ * gk_prefill_plan_build_two_way take two_way[n_seq], the number of leading tokens of each sequence that
+ * all of its rows see (0 = causal; at most the sequence's last position + 1, so that every such key is
+ * in the pool), for which row_limits[row] = max(position, two_way - 1).
+ * parts_before: see the shared prefix below; NULL = none. */
+GK_API int gk_paged_attn_extended_multi_bf16(
+    const void* q, int64_t q_row_stride, const void* new_k, const void* new_v, int64_t new_k_row_stride,
+    int64_t new_v_row_stride, const int32_t* locations, void* pool_k, void* pool_v, int64_t slots,
+    const int32_t* table, int64_t table_stride, int64_t table_entry_stride, int page_tokens,
+    const int32_t* table_rows, const int32_t* work, int64_t n_work, void* const* outs, int n_outs,
+    int64_t out_row_stride, float* part_ml, float* part_o, int32_t* split_counters, const float* slopes,
+    const int32_t* row_limits, const int32_t* parts_before, float scale, float softcap, int window,
+    int q_heads, int kv_heads, int head_dim, int32_t* status, gk_stream_t stream);
+GK_API int gk_paged_prefill_tc_biased_multi_bf16(
+    const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v, int64_t slots,
+    const int32_t* table, int64_t table_stride, int64_t table_entry_stride, int page_tokens,
+    const int32_t* table_rows, const int32_t* work, int64_t n_work, void* const* outs, int n_outs,
+    int64_t out_row_stride, const float* slopes, const int32_t* row_limits, float scale, float softcap,
+    int window, int q_heads, int kv_heads, int head_dim, int32_t* status, gk_stream_t stream);
+GK_API int gk_prefill_plan_build_two_way(const int32_t* seq, int64_t n_seq, const int32_t* two_way, int q_heads,
+                                  int kv_heads, int window, int min_rows, int32_t* work_out,
+                                  int64_t work_cap, int64_t* n_work_out, int32_t* rest_seq_out,
+                                  int64_t* n_rest_out);
+
+/* ---- prefixes that several sequences share ---------------------------------------------------------
+ * No counterpart in the reference.  Sequences of one group hold the same slots in their first
+ * prefix_tokens[group] positions (a common system prompt, several samples of one prompt).  The plan
+ * cuts every member's own work at the end of the prefix and adds records that attend to the prefix
+ * once for all rows of the group; their states (m, l, O) are merged with the members' own by the
+ * attention kernel, in a fixed order.
+ *   seq, two_way  as above (two_way may be NULL); groups[n_seq]: group of each sequence or -1;
+ *                 every member's first position lies at or behind the end of its group's prefix.
+ *   min_saved_bytes   a group is attended to together when that saves at least so much reading.
+ *   prefix_split_tokens  longest piece of a prefix per CTA, 0 = chosen from sm_count.
+ *   work_out, combine_out, partial_entries_out  as in gk_attention_plan_build; the low half of a
+ *                 record's last word counts the states in front too.
+ *   prefix_work_out  [cap*GK_WORK_WORDS] {first listed row, n_rows <= GK_PREFILL_TILES_PER_ITEM *
+ *                 (GK_PREFILL_TILE_ROWS / group), part, table_row, kv_begin, kv_end, largest position, 0}
+ *   prefix_rows_out  [cap*4] {row, position, entry of query head 0, entries between two parts}; the
+ *                 table row of a record is its group's first member's.
+ * Pass work_out == NULL to obtain the counts only.
+ *
+ * gk_shared_prefix_attn_bf16 runs the prefix records on the tensor cores (the kernel of
+ * gk_paged_prefill_tc_bf16, its rows gathered) and leaves their states in part_ml / part_o.  Then
+ * gk_paged_attn_extended_multi_bf16 with parts_before[row] = parts of the row's prefix (0 = none) and
+ * split_counters attends to the rest and merges.
+ * gk_shared_prefix_check compares table rows: pairs[n_pairs*4] = {row of the group's first member, row
+ * of another member, tokens, sequence} (rows through table_rows when not NULL); *verdict receives the
+ * smallest sequence that differs (-1: none) and GK_DEV_BAD_METADATA is raised for it. */
+GK_API int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, const int32_t* two_way,
+                                const int32_t* groups, const int32_t* prefix_tokens, int64_t n_groups,
+                                int q_heads, int kv_heads, int head_dim, int window, int sm_count,
+                                int split_tokens, int prefix_split_tokens, int64_t min_saved_bytes,
+                                int32_t* work_out, int64_t work_cap, int64_t* n_work_out,
+                                int32_t* combine_out, int64_t combine_cap, int64_t* n_combine_out,
+                                int64_t* partial_entries_out, int32_t* prefix_work_out,
+                                int64_t prefix_work_cap, int64_t* n_prefix_work_out,
+                                int32_t* prefix_rows_out, int64_t prefix_rows_cap,
+                                int64_t* n_prefix_rows_out);
+GK_API int gk_shared_prefix_attn_bf16(const void* q, int64_t q_row_stride, const void* pool_k,
+                               const void* pool_v, int64_t slots, const int32_t* table,
+                               int64_t table_stride, int64_t table_entry_stride, int page_tokens,
+                               const int32_t* table_rows, const int32_t* prefix_work,
+                               int64_t n_prefix_work, const int32_t* prefix_rows, float* part_ml,
+                               float* part_o, const float* slopes, float scale, float softcap, int window,
+                               int q_heads, int kv_heads, int head_dim, int32_t* status,
+                               gk_stream_t stream);
+GK_API int gk_shared_prefix_check(const int32_t* table, int64_t n_requests, int64_t context, int64_t table_stride,
+                           const int32_t* table_rows, int64_t n_table_rows, const int32_t* pairs,
+                           int64_t n_pairs, int32_t* verdict, int32_t* status, gk_stream_t stream);
+
 /* ---- tensor-parallel output gather fused into the attention epilogue ----------------------
  * Replaces AllGatherDimLast after attention (src/bridge/segmented_runner.cpp:170-191,
  * src/bridge/communicator.cpp:56-116: hcclAllGather into scratch + a transpose recipe): with KV
@@ -340,6 +418,28 @@ GK_API int gk_paged_slots_allocate(const int64_t* last_slots, const int64_t* fre
                             int64_t table_row_count, int64_t table_stride, int64_t table_context,
                             const int32_t* table_rows, int32_t* locations_out, int32_t* status,
                             gk_stream_t stream);
+
+/* The slots, table rows and index vectors of a step from lengths that live on the device (the host-list
+ * form is gk_paged_slots_layout + gk_paged_slots_allocate; no counterpart in the reference).  Request i
+ * of the batch holds lengths[i] cached tokens in table[requests[i]] and appends new_tokens[i]: its rows
+ * continue the open page behind the slot of its last cached token, then take fresh pages
+ * free_pages[*used_pages ...] in batch order.  Writes, per row in batch order, the slot, the position
+ * and the request (and the slot into the table); row_offsets[batch + 1]; next_lengths = lengths +
+ * new_tokens; *next_used = *used_pages + pages taken.  Rows past the last new token (up to `rows`) hold
+ * -1.  A batch that cannot be served whole -- a request out of range or named twice, a length that
+ * leaves the table, more new tokens than `rows`, too few free pages -- changes nothing: every row -1,
+ * offsets 0, next_* equal to the inputs, GK_DEV_BAD_METADATA.  A row whose page id (GK_DEV_BAD_SLOT) or
+ * whose last cached slot (GK_DEV_BAD_TABLE) is impossible gets slot -1 and no table cell.
+ * batch <= 65536, n_requests <= 262144 (GK_ERR_UNSUPPORTED).  `workspace`: 8-byte aligned device memory
+ * of gk_extend_requests_workspace_bytes bytes (0 up to 4096 requests). */
+GK_API int gk_extend_requests_workspace_bytes(int64_t batch, uint64_t* bytes_out);
+GK_API int gk_extend_requests(int32_t* table, int64_t n_requests, int64_t context, int64_t table_stride,
+                       const int32_t* requests, const int64_t* lengths, const int32_t* new_tokens,
+                       int64_t batch, const int64_t* free_pages, int64_t n_free,
+                       const int64_t* used_pages, int64_t page_size, int64_t rows, void* workspace,
+                       int32_t* locations, int32_t* positions, int32_t* row_requests,
+                       int32_t* row_offsets, int64_t* next_lengths, int64_t* next_used, int32_t* status,
+                       gk_stream_t stream);
 
 /* Slot release, replaces gk_paged_free_i32_v1 (src/bridge/paged_slot_allocator.cpp:153-209):
  * pages_out receives slot / page_size for every slot, in order of first occurrence, each page
