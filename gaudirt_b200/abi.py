@@ -39,13 +39,14 @@ PROTOTYPES = {
                                        f32, i32, i32, i32, i32, vp, vp]),
     "gk_paged_attn_combine_multi_bf16": (i32, [vp, vp, vp, i64, vp, i32, i64, i32, i32, vp]),
     "gk_prefill_plan_build_two_way": (i32, [vp, i64, vp, i32, i32, i32, i32, vp, i64, i64p, vp, i64p]),
-    "gk_shared_prefix_plan_build": (i32, [vp, i64, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, i64, vp, i64, i64p,
-                                          vp, i64, i64p, i64p, vp, i64, i64p, vp, i64, i64p]),
+    "gk_shared_prefix_plan_build": (i32, [vp, i64, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, i64, C.POINTER(i32),
+                                          vp, i64, i64p, vp, i64, i64p, i64p, vp, i64, i64p, vp, i64, i64p]),
     "gk_shared_prefix_check": (i32, [vp, i64, i64, i64, vp, i64, vp, i64, vp, vp, vp]),
-    "gk_shared_prefix_attn_bf16": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64, vp, vp, vp, vp, f32, f32, i32,
+    "gk_shared_prefix_attn_bf16": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64, i32, vp, vp, vp, vp, f32, f32, i32,
                                          i32, i32, i32, vp, vp]),
     "gk_paged_attn_extended_multi_bf16": (i32, [vp, i64, vp, vp, i64, i64, vp, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64,
-                                                vp, i32, i64, vp, vp, vp, vp, vp, vp, f32, f32, i32, i32, i32, i32, vp, vp]),
+                                                vp, i32, i64, vp, vp, vp, vp, vp, vp, i32, f32, f32, i32, i32, i32, i32, vp,
+                                                vp]),
     "gk_paged_prefill_tc_biased_multi_bf16": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64, vp, i32, i64, vp,
                                                     vp, f32, f32, i32, i32, i32, i32, vp, vp]),
     "gk_peer_barrier": (i32, [vp, i32, i32, i32, i64, vp, vp]),

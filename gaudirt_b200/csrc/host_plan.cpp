@@ -385,20 +385,21 @@ extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_
 extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, const int32_t* two_way, const int32_t* groups,
                                            const int32_t* prefix_tokens, int64_t n_groups, int q_heads, int kv_heads,
                                            int head_dim, int window, int sm_count, int split_tokens,
-                                           int prefix_split_tokens, int64_t min_saved_bytes, int32_t* work_out,
+                                           int prefix_split_tokens, int64_t min_saved_bytes, int* form_out,
+                                           int32_t* work_out,
                                            int64_t work_cap, int64_t* n_work_out, int32_t* combine_out,
                                            int64_t combine_cap, int64_t* n_combine_out, int64_t* partial_entries_out,
                                            int32_t* prefix_work_out, int64_t prefix_work_cap, int64_t* n_prefix_work_out,
                                            int32_t* prefix_rows_out, int64_t prefix_rows_cap, int64_t* n_prefix_rows_out) {
   if (!seq || n_seq <= 0 || n_groups < 0 || (n_groups > 0 && (!groups || !prefix_tokens)) || prefix_split_tokens < 0 ||
-      min_saved_bytes < 0 || !n_prefix_work_out || !n_prefix_rows_out || sm_count <= 0 || (window != -1 && window <= 0))
+      min_saved_bytes < 0 || !form_out || !n_prefix_work_out || !n_prefix_rows_out || sm_count <= 0 || (window != -1 && window <= 0))
     return GK_ERR_INVALID_ARGUMENT;
   if (q_heads <= 0 || q_heads > 256 || kv_heads <= 0 || kv_heads > 256 || q_heads % kv_heads != 0 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256) || q_heads / kv_heads > GK_MAX_PACKED_ROWS)
     return GK_ERR_UNSUPPORTED;
   const int group_heads = q_heads / kv_heads;
   const int tile = head_dim == 256 ? 64 : 128;                                    // keys of one tile of the kernel
-  const int record_rows = GK_PREFILL_TILES_PER_ITEM * (GK_PREFILL_TILE_ROWS / group_heads);
+  const int tile_rows = GK_PREFILL_TILE_ROWS / group_heads;
   const int ctas_per_record = head_dim == 256 ? 2 : 1;
 
   struct Group { std::vector<int32_t> members; int64_t rows = 0; int32_t lo = 0, hi = 0; };
@@ -415,9 +416,10 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
     all[g].members.push_back((int32_t)s);
     all[g].rows += r[1];
   }
-  // A group is attended to together when that saves enough reading to pay for the launch and for the merge of its parts.
+  // Groups are attended to together when that saves enough reading to pay for the launch and for the merge of the parts.
   std::vector<Group*> shared;
   const int64_t token_bytes = (int64_t)kv_heads * head_dim * 4;
+  int64_t saved = 0;
   for (int64_t g = 0; g < n_groups; ++g) {
     Group& one = all[g];
     one.hi = prefix_tokens[g];
@@ -425,27 +427,39 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
     for (int32_t s : one.members)
       one.lo = std::min(one.lo, window > 0 ? std::max(0, seq[s * 4 + 2] - window + 1) : 0);   // first key any row sees
     if (one.members.size() < 2 || one.hi <= one.lo) continue;
+    saved += (int64_t)(one.members.size() - 1) * (one.hi - one.lo) * token_bytes;
     one.lo = one.lo / tile * tile;                                   // whole tiles: a row's own window is masked in the kernel
-    if ((int64_t)(one.members.size() - 1) * (one.hi - one.lo) * token_bytes < min_saved_bytes) continue;
     shared.push_back(&one);
   }
+  if (saved < min_saved_bytes) shared.clear();
+  // Records of one query tile keep two chains of products going and wait less (0.98 us for a 128-row tile and 128 keys,
+  // 2.3 us for two tiles together), records of two fetch every key tile for twice as many rows.  Measured at head_dim 128:
+  // one tile 4-8 % faster at up to 14 tile products per SM, two tiles 2-6 % faster at 55 and 110.
+  int64_t most_rows = 0, products = 0;
+  for (const Group* g : shared) {
+    most_rows = std::max(most_rows, g->rows);
+    products += (g->rows + tile_rows - 1) / tile_rows * ((g->hi - g->lo + tile - 1) / tile) * kv_heads;
+  }
+  const bool one_tile = head_dim != 256 && !shared.empty() && (most_rows <= tile_rows || products < 32 * (int64_t)sm_count);
+  const int record_rows = one_tile ? tile_rows : GK_PREFILL_TILES_PER_ITEM * tile_rows;
   // How long a piece of the prefix one CTA takes: the cheapest of the whole-tile lengths, by the time the CTAs need on
-  // sm_count SMs (one CTA each), in units of one key tile against two query tiles.  A CTA costs its tiles and a fixed
-  // prologue and epilogue; every piece leaves (m, l, O) states that are written and read once more.
+  // sm_count SMs (one CTA each), in units of one key tile.  A CTA costs its tiles and a fixed prologue and
+  // epilogue; every piece leaves (m, l, O) states that are written and read once more.
   int64_t piece = prefix_split_tokens;
   if (piece == 0 && !shared.empty()) {
     int32_t longest = 0;
     for (const Group* g : shared) longest = std::max(longest, g->hi - g->lo);
-    constexpr double kCtaTiles = 2.5, kStateTiles = 0.2;
+    const double kCtaTiles = one_tile ? 7.0 : 3.0;                // 7-8 us
+    constexpr double kPartTiles = 0.15;                           // what one more part costs a row's merge
     double best = 0.0;
     for (int64_t tiles = 1; tiles <= (longest + tile - 1) / tile; tiles = tiles < 16 ? tiles + 1 : tiles + tiles / 8) {
       std::vector<int32_t> costs;                                 // tiles per CTA; the scheduler takes them in order
-      double states = 0.0;
+      int64_t most_parts = 0;
       for (const Group* g : shared) {
         const int64_t records = (g->rows + record_rows - 1) / record_rows * kv_heads * ctas_per_record;
         const int64_t span = (g->hi - g->lo + tile - 1) / tile, pieces = (span + tiles - 1) / tiles;
         const int64_t even = (span + pieces - 1) / pieces;
-        states += (double)(pieces * records);
+        most_parts = std::max(most_parts, pieces);
         if (pieces * records > 16 * (int64_t)sm_count) { costs.clear(); break; }
         for (int64_t i = 0; i < pieces; ++i)
           for (int64_t k = 0; k < records; ++k) costs.push_back((int32_t)std::min<int64_t>(even, span - i * even));
@@ -465,7 +479,7 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
         makespan = std::max(makespan, heap.back());
         std::push_heap(heap.begin(), heap.end(), later);
       }
-      const double cost = makespan + kStateTiles * states / sm_count;
+      const double cost = makespan + kPartTiles * (double)most_parts;
       if (piece == 0 || cost < best) {
         best = cost;
         piece = tiles * tile;
@@ -508,6 +522,14 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
                                          work_out, work_cap, n_work_out, combine_out, combine_cap, n_combine_out,
                                          partial_entries_out);
   if (built != GK_OK) return built;
+  // Tails of one query block each, many of them and short: two warps and four CTAs per SM instead of four warps and two,
+  // so that a CTA's fixed cost (3 to 4 us of look-ups and merges) is a smaller part of its time.  Measured at head_dim 128:
+  // 10-14 % faster at 1024 and 2048 CTAs of 64 to 512 tokens, even at 8192 tokens, 10-25 % slower at 128 to 512 CTAs.
+  int64_t own_tokens = 0;
+  for (int64_t s = 0; s < n_seq; ++s) own_tokens += seq[s * 4 + 2] + seq[s * 4 + 1] - kv_from[s];
+  const bool short_tails = head_dim != 256 && !items.empty() && *n_work_out * kv_heads >= 6 * (int64_t)sm_count &&
+                           own_tokens <= 2048 * *n_work_out;
+  *form_out = (one_tile ? GK_SHARED_ONE_TILE : 0) | (short_tails ? GK_SHARED_SHORT_TAILS : 0);
   *n_prefix_work_out = (int64_t)items.size();
   *n_prefix_rows_out = (int64_t)rows.size();
   if (!work_out) return GK_OK;

@@ -89,7 +89,7 @@ struct PrefillParams {
 };
 
 struct Shared {
-  uint64_t k_full[kKStages], k_free[kKStages], v_full[kVStages], v_free[kVStages];
+  uint64_t k_full[kKStages + 1], k_free[kKStages + 1], v_full[kVStages], v_free[kVStages];
   uint64_t s_full[2], p_full[2], pv_done[2];
   uint32_t tmem_base;
   int abort;
@@ -135,11 +135,27 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// BIASED: a distance bias and row limits.  SHARED: the rows of a record are listed (they belong to several sequences
-// that share the keys of the record), every listed row sees all of the record's keys but for its window, and the state
-// (m, l, O) is left for the merge instead of a normalised row.  A record of the shared form is {first listed row,
-// n_rows, part, table_row, kv_begin, kv_end, largest position, 0}.
-template <int D, bool BIASED, bool SHARED>
+// softcap * tanh(scale * s / softcap) in log2 units, from tanh(x) = 1 - 2 / (exp(2x) + 1): `e` is 2 log2(e) scale / softcap
+// and `c` softcap * log2(e).  Both ends come out exactly (exp2 gives 0 or infinity).  The absolute error is a few 2^-22 of
+// the cap (three fp32 operations on values of at most 2), next to which a probability's rounding to bf16 is 2^-9; a score
+// enters an exponential, so its absolute error is what counts, not the relative one near zero.
+__device__ __forceinline__ float capped_score(float s, float e, float c) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(fast_exp2(s * e) + 1.f));
+  return fmaf(-2.f * c, r, c);
+}
+
+// BIASED: a distance bias and row limits.
+// FORM: kRowsForm is the kernel described above.  The shared forms attend to keys that several sequences have in common:
+// the rows of a record are listed, every listed row sees all of the record's keys but for its window, and the state
+// (m, l, O) is left for the merge instead of a normalised row.  A record is {first listed row, n_rows, part, table_row,
+// kv_begin, kv_end, largest position, 0}.  kWideForm takes two query tiles like kRowsForm.  kNarrowForm (head_dim 64 and
+// 128) takes one: its even KV tiles are the work of softmax warps 0-3, S0 and O0, its odd ones of warps 4-7, S1 and O1, so
+// the tensor pipe still has two independent chains although a K/V tile is read for one query tile only, Q.K^T runs two KV
+// tiles ahead, and the room of the second query tile is a third K stage; the two chains' states are merged through shared
+// memory at the end.
+constexpr int kRowsForm = 0, kWideForm = 1, kNarrowForm = 2;
+template <int D, bool BIASED, int FORM>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const PrefillParams p,
                                                                        const __grid_constant__ CUtensorMap map_k,
                                                                        const __grid_constant__ CUtensorMap map_v) {
@@ -148,10 +164,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   constexpr int kQPanelBytes = G_::kQPanelBytes, kQTileBytes = G_::kQTileBytes;
   constexpr int kKvPanelBytes = G_::kKvPanelBytes, kKvTileBytes = G_::kKvTileBytes;
   constexpr int kScoreChunks = kKv / 32;                 // 32-column pieces of a row of S
+  constexpr bool SHARED = FORM != kRowsForm, NARROW = FORM == kNarrowForm;
+  static_assert(!NARROW || kTiles == 2, "the narrow form needs room for two accumulators in tensor memory");
+  constexpr int kQTiles = NARROW ? 1 : kTiles, kKRing = NARROW ? kKStages + 1 : kKStages;
   extern __shared__ __align__(1024) uint8_t tiles[];     // swizzle atoms need 1 KiB alignment
   uint8_t* s_q = tiles;                                  // the query tiles
-  uint8_t* s_k = s_q + kTiles * kQTileBytes;             // K stages
-  uint8_t* s_v = s_k + kKStages * kKvTileBytes;          // V stages
+  uint8_t* s_k = s_q + kQTiles * kQTileBytes;            // K stages
+  uint8_t* s_v = s_k + kKRing * kKvTileBytes;            // V stages
   Shared* sh = reinterpret_cast<Shared*>(s_v + kVStages * kKvTileBytes);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -181,15 +200,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       if (p.window > 0) kv_begin = max(kv_begin, first_pos - p.window + 1);
     }
   }
-  const int rows0 = min(n_rows, tile_rows), rows1 = n_rows - rows0;
+  const int rows0 = min(n_rows, tile_rows), rows1 = NARROW ? rows0 : n_rows - rows0;
+  const int tile_step = NARROW ? 0 : tile_rows;             // rows between the two tiles (chains)
   // KV tiles each query tile needs: tile 0 stops at its own last row (causal), tile 1 at the record's end
   const int nt1_all = (kv_end - kv_begin + kKv - 1) / kKv;
-  const int nt0 = SHARED ? nt1_all : min(nt1_all, (last_seen(first_row + rows0 - 1, first_pos + rows0 - 1) + 1 - kv_begin + kKv - 1) / kKv);
-  const int nt1 = rows1 > 0 ? nt1_all : 0;
-  const int n_tiles = max(nt0, nt1);
+  const int nt0 = NARROW ? (nt1_all + 1) / 2 : SHARED ? nt1_all : min(nt1_all, (last_seen(first_row + rows0 - 1, first_pos + rows0 - 1) + 1 - kv_begin + kKv - 1) / kKv);
+  const int nt1 = NARROW ? nt1_all / 2 : rows1 > 0 ? nt1_all : 0;
+  const int n_tiles = NARROW ? nt1_all : max(nt0, nt1);
+  // Under a distance bias the nearest keys weigh most: the biased kernel walks the KV range backwards, so that the running
+  // maximum is there after the first tile.  Forwards it grew with every tile, and each time O was rescaled in tensor
+  // memory behind a wait for the product before (12 % of the launch).  A query tile whose range ends earlier then starts
+  // later: its first KV tile is number `head0`.
+  const int head0 = BIASED && !NARROW ? n_tiles - nt0 : 0;
+  auto tile_at = [&](int j) { return kv_begin + (BIASED ? n_tiles - 1 - j : j) * kKv; };
 
   if (tid == 0) {
-    for (int i = 0; i < kKStages; ++i) {
+    for (int i = 0; i < kKRing; ++i) {
       bar_init(&sh->k_full[i], kLoaderThreads);
       bar_init(&sh->k_free[i], 1);
     }
@@ -209,6 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh->tmem_base)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
   }
+  // The shared forms may be set up while the kernel before them runs.  The attention kernel behind them is released only
+  // once that kernel has completed: it reads the queries and the pool without waiting for this one.
+  if (SHARED) asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;\n" ::: "memory");
   tc_fence_before();
   __syncthreads();                                       // barriers and the TMEM allocation are in place
   tc_fence_after();
@@ -216,25 +245,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   if (!is_loader) {
     // Q tiles: packed row pr of tile t = (row t*tile_rows + pr / G, query head pr % G) of this KV head; unused rows
     // are zero.  The loader warps do not take part: their first K/V tiles are already on the way meanwhile.
-    const int filler = warp < 8 ? tid : tid - 128;       // 0..383
-    for (int i = filler; i < kTiles * kRows * kChunks; i += kThreads - 128) {
-      const int t = i / (kRows * kChunks), pr = (i / kChunks) & (kRows - 1), c = i & (kChunks - 1);
-      uint4 v = make_uint4(0, 0, 0, 0);
-      const int r = t * tile_rows + pr / G, g = pr % G;
-      if (pr < tile_rows * G && r < n_rows) {
-        const int row = SHARED ? __ldg(&p.list[first_row + r].x) : first_row + r;
-        const __nv_bfloat16* src = p.q + (int64_t)row * p.q_stride + (int64_t)(head * G + g) * D + c * 8;
-        if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-          v = __ldg(reinterpret_cast<const uint4*>(src));
-        } else {
-          const unsigned short* s16 = reinterpret_cast<const unsigned short*>(src);
-          unsigned short e[8];
+    // Warps 0-7 take kQTiles * 16 rows each: a lane finds the place of one row (one division, one look at the list), then
+    // the warp copies the rows in turn, 512 bytes an instruction, all of them under way at once.
+    if (warp < 8) {
+      constexpr int kWarpRows = kQTiles * 16, kRowsAtOnce = 32 / kChunks;
+      const bool q_aligned = ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)(p.q_stride * 2)) & 15) == 0;
+      int64_t place = -1;                                  // of the row warp * kWarpRows + lane, in elements of q
+      {
+        const int at = warp * kWarpRows + lane, t = at / kRows, pr = at & (kRows - 1), r = t * tile_rows + pr / G;
+        if (lane < kWarpRows && pr < tile_rows * G && r < n_rows)
+          place = (int64_t)(SHARED ? __ldg(&p.list[first_row + r].x) : first_row + r) * p.q_stride + (int64_t)(head * G + pr % G) * D;
+      }
+      const int c = lane & (kChunks - 1);
+      auto target = [&](int at) { return s_q + (at / kRows) * kQTileBytes + tile_off(at & (kRows - 1), c, kQPanelBytes); };
+      if (q_aligned) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) e[k] = __ldg(s16 + k);
-          v = *reinterpret_cast<const uint4*>(e);
+        for (int i = 0; i < kWarpRows; i += kRowsAtOnce) {
+          const int64_t from = __shfl_sync(0xffffffffu, place, i + lane / kChunks);
+          cp_async_16(smem_u32(target(warp * kWarpRows + i + lane / kChunks)), p.q + (from < 0 ? 0 : from + c * 8), from < 0 ? 0 : 16);
+        }
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kWarpRows; i += kRowsAtOnce) {
+          const int64_t from = __shfl_sync(0xffffffffu, place, i + lane / kChunks);
+          unsigned short* dst = reinterpret_cast<unsigned short*>(target(warp * kWarpRows + i + lane / kChunks));
+          const unsigned short* src = reinterpret_cast<const unsigned short*>(p.q) + (from < 0 ? 0 : from + c * 8);
+#pragma unroll 1
+          for (int k = 0; k < 8; ++k) dst[k] = from < 0 ? 0 : __ldg(src + k);
         }
       }
-      *reinterpret_cast<uint4*>(s_q + t * kQTileBytes + tile_off(pr, c, kQPanelBytes)) = v;
     }
     fence_async_smem();
     asm volatile("bar.sync 1, %0;\n" ::"n"(kThreads - 128) : "memory");      // the 384 threads that filled Q
@@ -266,16 +306,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     const int my_rows = t == 0 ? rows0 : rows1;
     const int mv = my_rows * G;                                  // packed rows of this tile in use
     const int my_tiles = t == 0 ? nt0 : nt1;
-    const int tile_first_pos = first_pos + t * tile_rows;
+    const int tile_first_pos = first_pos + t * tile_step;
     int lim = pr < mv ? tile_first_pos + pr / G : 0x7fffffff;         // last visible key of this row
     int pos = lim;                                                     // its position
     int4 listed = make_int4(0, 0, 0, 0);
     if (SHARED) {
-      if (pr < mv) listed = __ldg(p.list + first_row + t * tile_rows + pr / G);
+      if (pr < mv) listed = __ldg(p.list + first_row + t * tile_step + pr / G);
       pos = pr < mv ? listed.y : 0x7fffffff;
       lim = 0x7fffffff;
     } else if (BIASED && pr < mv) {
-      lim = last_seen(first_row + t * tile_rows + pr / G, pos);
+      lim = last_seen(first_row + t * tile_step + pr / G, pos);
     }
     // bias per token of distance, in log2 units
     const float slope = BIASED && p.slopes && pr < mv ? __ldg(p.slopes + head * G + pr % G) * kLog2e : 0.f;
@@ -284,6 +324,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     const bool capped = p.softcap > 0.f;
     const float to_log2 = capped ? kLog2e : p.scale * kLog2e;
     const float cap_in = capped ? p.scale / p.softcap : 0.f;
+    const float cap_exp = 2.f * kLog2e * cap_in, cap_log2 = p.softcap * kLog2e;     // see capped_score
+    const bool steep = BIASED && __any_sync(0xffffffffu, fabsf(slope) * 31.f > 100.f);
     float m = -CUDART_INF_F, l = 0.f;                            // m: exponent reference of this row
     bool alive = true;
     for (int j = 0; j < my_tiles && alive; ++j) {
@@ -296,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       alive = __all_sync(0xffffffffu, bar_wait(&sh->s_full[buf], use & 1, &sh->abort));
       if (!alive) break;
       tc_fence_after();
-      const int tok0 = kv_begin + j * kKv;
+      const int tok0 = tile_at(NARROW ? 2 * j + t : t == 0 ? j + head0 : j);
       const int tile_end = tok0 + kKv;
       const bool ragged = SHARED ? tile_end > kv_end || (p.window > 0 && tok0 <= w1.z - p.window)
                                  : tile_end > kv_end || tile_end > tile_first_pos + 1 ||
@@ -307,7 +349,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       // the two passes below stay one short piece of code (the instruction cache is what this kernel
       // runs out of first when every variant is unrolled 128 times).
       float mult = to_log2;
-      if (capped || ragged) {
+      // Slopes too steep for the estimate of the maximum below go the exact way of the uncommon tiles.
+      const bool rewrite = capped || ragged || (BIASED && steep);
+      const float fast_slope = BIASED && !rewrite ? slope : 0.f;
+      if (rewrite) {
+        if (BIASED || SHARED) {
+          // The keys a row sees are one interval: a key is in it when its distance from the first one is at most `span`.
+          int low = p.window > 0 ? pos - p.window + 1 : 0, span = min(lim, kv_end - 1) - low;
+          if (span < 0) {                               // no key at all: an interval in front of every tile
+            low = 0x7fffffff;
+            span = 0;
+          }
+          const int rel = tok0 - low;
+#pragma unroll 1
+          for (int c = 0; c < kScoreChunks; ++c) {
+            uint32_t r[32];
+            tmem_ld32(s_addr + c * 32, r);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float v = __uint_as_float(r[e]);
+              v = capped ? capped_score(v, cap_exp, cap_log2) : v * to_log2;
+              if (BIASED) v = fmaf(-slope, fabsf(from + (float)(c * 32 + e)), v);
+              r[e] = __float_as_uint((unsigned)(rel + c * 32 + e) <= (unsigned)span ? v : -CUDART_INF_F);
+            }
+            tmem_st32(s_addr + c * 32, r);
+          }
+        } else {
 #pragma unroll 1
         for (int c = 0; c < kScoreChunks; ++c) {
           uint32_t r[32];
@@ -324,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
           }
           tmem_st32(s_addr + c * 32, r);
         }
+        }
         mult = 1.f;
       }
       // ---- the whole row comes in once (up to 128 registers) and stays until it has become P ----
@@ -331,20 +399,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
 #pragma unroll
       for (int c = 0; c < kScoreChunks; ++c) tmem_ld32_nowait(s_addr + c * 32, sr[c]);
       tmem_ld_wait();
-      if (BIASED && !(capped || ragged)) {
-        // every key of an unmasked tile is at or before the row's position: -slope * |distance| = slope * (from + e)
-        const float2 slope2 = make_float2(slope, slope), first2 = make_float2(slope * from, slope * from), mult_in = make_float2(mult, mult);
-#pragma unroll
-        for (int c = 0; c < kScoreChunks; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 bias = __ffma2_rn(slope2, make_float2((float)(c * 32 + e), (float)(c * 32 + e + 1)), first2);
-            const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), mult_in, bias);
-            sr[c][e] = __float_as_uint(x.x);
-            sr[c][e + 1] = __float_as_uint(x.y);
-          }
-        mult = 1.f;
-      }
       float mx;
       {
         float part[kScoreChunks];
@@ -356,9 +410,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
           for (int c = 0; c < kScoreChunks; ++c)
             part[c] = max3(part[c], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
         }
+        if (BIASED) {
+          // Every key of an unmasked tile is at or before the row's position: its bias is slope * (from + e).  The
+          // reference of the exponent is taken from the raw maxima of 32 columns and the larger of their two end biases:
+          // it lies above the true maximum by at most 31 slopes, under 2^100 of range (see `steep`), which costs nothing
+          // in fp32 or bf16 and saves the biased scores a pass of their own.
+#pragma unroll
+          for (int c = 0; c < kScoreChunks; ++c) {
+            const float first = fast_slope * (from + (float)(c * 32));
+            part[c] = fmaf(part[c], mult, fmaxf(first, first + 31.f * fast_slope));
+          }
+        }
         mx = fmaxf(part[0], part[1]);
         if (kScoreChunks == 4) mx = fmaxf(mx, fmaxf(part[2], part[3]));
-        mx *= mult;                                                                 // mult > 0
+        if (!BIASED) mx *= mult;                                                    // mult > 0
       }
       // The exponent reference only moves when the maximum grew by more than 2^8: P stays within
       // bf16/fp32 range and O needs rescaling (and the wait for the previous P.V) only then.
@@ -390,9 +455,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
 #pragma unroll
       for (int c = 0; c < kScoreChunks; ++c) {
         uint32_t packed[16];
+        // the biases of two neighbouring keys, stepped by additions within 32 columns (at most 16 roundings)
+        float2 addend = neg_mu2;
+        const float2 bias_step = make_float2(2.f * fast_slope, 2.f * fast_slope);
+        if (BIASED) {
+          const float first = fast_slope * (from + (float)(c * 32)) - mu;
+          addend = make_float2(first, first + fast_slope);
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), mult2, neg_mu2);
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), mult2, addend);
+          if (BIASED) addend = __fadd2_rn(addend, bias_step);
           const float2 pr2 = make_float2(fast_exp2(x.x), fast_exp2(x.y));
           sum2[i & 1] = __fadd2_rn(sum2[i & 1], pr2);
           packed[i] = pack_bf16(pr2.x, pr2.y);
@@ -405,44 +478,94 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       __syncwarp();                                      // every lane's P is in tensor memory: one arrival per warp
       if (lane == 0) bar_arrive(&sh->p_full[buf]);
     }
-    // epilogue: O / l -> bf16 rows of the output
-    if (alive && my_tiles > 0) {
-      alive = __all_sync(0xffffffffu, bar_wait(pv_bar(t, my_tiles - 1), pv_phase(my_tiles - 1), &sh->abort));
+    // The row a thread owns leaves through shared memory, so that a warp stores whole rows: one thread storing its own
+    // row 16 bytes at a time touched 32 rows per instruction and took 3 us per CTA.  16-byte chunks are exchanged by row
+    // (^ row & 7), which keeps both sides free of bank conflicts.
+    if (SHARED) {
+      // wait for the products of both tiles (chains): nothing reads the K and V stages any more, they take the O rows
+      if (alive && my_tiles > 0) alive = __all_sync(0xffffffffu, bar_wait(pv_bar(t, my_tiles - 1), pv_phase(my_tiles - 1), &sh->abort));
+      const bool have = alive && my_tiles > 0;
+      tc_fence_after();
+      asm volatile("bar.sync 2, %0;\n" ::"n"(kSoftmaxThreads) : "memory");
+      constexpr int kRowChunks = D / 4;
+      float4* rows = reinterpret_cast<float4*>(s_k);
+      float2* states = reinterpret_cast<float2*>(s_k + kTiles * kRows * D * 4);
+      int* entries = reinterpret_cast<int*>(states + 2 * kRows);
+      static_assert(kTiles * kRows * D * 4 + 2 * kRows * 12 <= (kKRing + kVStages) * kKvTileBytes, "room for the rows");
+      states[t * kRows + pr] = make_float2(m, have ? l : 0.f);
+      entries[t * kRows + pr] = pr < mv ? listed.z + w0.z * listed.w + head * G + pr % G : -1;
+      if (t < kTiles) {
+#pragma unroll 1
+        for (int cb = 0; cb < D / 32; ++cb) {
+          uint32_t r[32];
+          if (have) {
+            tmem_ld32(o_addr + cb * 32, r);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[e] = 0;
+          }
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            rows[(t * kRows + pr) * kRowChunks + ((cb * 8 + c) ^ (pr & 7))] =
+                make_float4(__uint_as_float(r[c * 4]), __uint_as_float(r[c * 4 + 1]), __uint_as_float(r[c * 4 + 2]),
+                            __uint_as_float(r[c * 4 + 3]));
+        }
+      }
+      asm volatile("bar.sync 2, %0;\n" ::"n"(kSoftmaxThreads) : "memory");
+      // narrow: eight warps over the rows of the one tile, both chains merged; wide: four warps over the rows of each
+      for (int row = NARROW ? warp : warp & 3; row < mv; row += NARROW ? 8 : 4) {
+        const int at = NARROW ? row : t * kRows + row;
+        float2 state = states[at];
+        float w_a = 1.f, w_b = 0.f;
+        if (NARROW) {
+          const float2 other = states[kRows + row];
+          float top = state.y > 0.f ? state.x : -CUDART_INF_F;
+          if (other.y > 0.f) top = fmaxf(top, other.x);
+          w_a = state.y > 0.f ? fast_exp2(state.x - top) : 0.f;
+          w_b = other.y > 0.f ? fast_exp2(other.x - top) : 0.f;
+          state = make_float2(top, w_a * state.y + w_b * other.y);
+        }
+        const int64_t entry = entries[at];
+        if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + entry * 2) = state;
+        for (int c = lane; c < kRowChunks; c += 32) {
+          float4 o = rows[at * kRowChunks + (c ^ (row & 7))];
+          if (NARROW) {
+            const float4 x = rows[(kRows + row) * kRowChunks + (c ^ (row & 7))];
+            o = make_float4(w_a * o.x + w_b * x.x, w_a * o.y + w_b * x.y, w_a * o.z + w_b * x.z, w_a * o.w + w_b * x.w);
+          }
+          *reinterpret_cast<float4*>(p.part_o + entry * D + c * 4) = o;
+        }
+      }
+    } else if (my_tiles > 0) {
+      // epilogue: O / l -> bf16 rows of the output, through this tile's own query rows (its last Q.K^T has run)
+      if (alive) alive = __all_sync(0xffffffffu, bar_wait(pv_bar(t, my_tiles - 1), pv_phase(my_tiles - 1), &sh->abort));
+      uint4* rows = reinterpret_cast<uint4*>(s_q + t * kQTileBytes);
       if (alive) {
         tc_fence_after();
-        if (SHARED) {
-          const int64_t entry = (int64_t)listed.z + (int64_t)w0.z * listed.w + head * G + pr % G;
-          if (pr < mv) *reinterpret_cast<float2*>(p.part_ml + entry * 2) = make_float2(m, l);
-#pragma unroll 1
-          for (int cb = 0; cb < D / 32; ++cb) {
-            uint32_t r[32];
-            tmem_ld32(o_addr + cb * 32, r);
-            if (pr < mv) {
-#pragma unroll
-              for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<uint4*>(p.part_o + entry * D + cb * 32 + c * 4) = make_uint4(r[c * 4], r[c * 4 + 1], r[c * 4 + 2], r[c * 4 + 3]);
-            }
-          }
-        } else {
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        const int r_q = t * tile_rows + pr / G, g = pr % G;
-        const int64_t at = (int64_t)(first_row + r_q) * p.out_stride + (int64_t)(head * G + g) * D;
 #pragma unroll 1
         for (int cb = 0; cb < D / 32; ++cb) {
           uint32_t r[32];
           tmem_ld32(o_addr + cb * 32, r);
-          if (pr < mv) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint4 v;
-              v.x = pack_bf16(__uint_as_float(r[c * 8 + 0]) * inv, __uint_as_float(r[c * 8 + 1]) * inv);
-              v.y = pack_bf16(__uint_as_float(r[c * 8 + 2]) * inv, __uint_as_float(r[c * 8 + 3]) * inv);
-              v.z = pack_bf16(__uint_as_float(r[c * 8 + 4]) * inv, __uint_as_float(r[c * 8 + 5]) * inv);
-              v.w = pack_bf16(__uint_as_float(r[c * 8 + 6]) * inv, __uint_as_float(r[c * 8 + 7]) * inv);
-              for (int dst = 0; dst < p.n_out; ++dst) *reinterpret_cast<uint4*>(p.out[dst] + at + cb * 32 + c * 8) = v;
-            }
+          for (int c = 0; c < 4; ++c) {
+            uint4 v;
+            v.x = pack_bf16(__uint_as_float(r[c * 8 + 0]) * inv, __uint_as_float(r[c * 8 + 1]) * inv);
+            v.y = pack_bf16(__uint_as_float(r[c * 8 + 2]) * inv, __uint_as_float(r[c * 8 + 3]) * inv);
+            v.z = pack_bf16(__uint_as_float(r[c * 8 + 4]) * inv, __uint_as_float(r[c * 8 + 5]) * inv);
+            v.w = pack_bf16(__uint_as_float(r[c * 8 + 6]) * inv, __uint_as_float(r[c * 8 + 7]) * inv);
+            rows[pr * kChunks + ((cb * 4 + c) ^ (pr & 7))] = v;
           }
         }
+      }
+      asm volatile("bar.sync %0, 128;\n" ::"r"(2 + t) : "memory");         // the four warps of this tile
+      if (alive) {
+        constexpr int kRowsAtOnce = 32 / kChunks;
+        const int c = lane & (kChunks - 1);
+        for (int row = (warp & 3) * kRowsAtOnce + lane / kChunks; row < mv; row += 4 * kRowsAtOnce) {
+          const uint4 v = rows[row * kChunks + (c ^ (row & 7))];
+          const int64_t at = (int64_t)(first_row + t * tile_rows + row / G) * p.out_stride + (int64_t)(head * G + row % G) * D + c * 8;
+          for (int dst = 0; dst < p.n_out; ++dst) *reinterpret_cast<uint4*>(p.out[dst] + at) = v;
         }
       }
     }
@@ -450,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     // ================================ K/V loaders =========================================
     const bool is_v = warp >= 10;
     const int lwarp = (warp - 8) & 1;
-    const int stages = is_v ? kVStages : kKStages;
+    const int stages = is_v ? kVStages : kKRing;
     const __nv_bfloat16* base = (is_v ? p.pool_v : p.pool_k) + (int64_t)head * p.slots * D;
     const int32_t* trow = p.table + (int64_t)(p.table_rows ? __ldg(p.table_rows + table_row) : table_row) * p.table_stride;
     const int page_mask = (1 << p.page_shift) - 1;
@@ -464,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       int slot[kHalves];
 #pragma unroll
       for (int half = 0; half < kHalves; ++half) {
-        const int tok = kv_begin + j * kKv + lwarp * kWarpRows + half * 32 + lane;
+        const int tok = tile_at(j) + lwarp * kWarpRows + half * 32 + lane;
         slot[half] = -1;
         if (tok < kv_end) {
           slot[half] = __ldg(trow + (int64_t)(tok >> p.page_shift) * p.entry_stride) + (tok & page_mask);
@@ -476,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       }
       // This warp's rows go by TMA when they are whole, in-range boxes of tma_rows slot-contiguous
       // tokens; the two warps of a tile decide independently (every thread arrives once either way).
-      const int tok_first = kv_begin + j * kKv + lwarp * kWarpRows;
+      const int tok_first = tile_at(j) + lwarp * kWarpRows;
       bool by_tma = p.tma_rows > 0 && (tok_first & (p.tma_rows - 1)) == 0 && tok_first + kWarpRows <= kv_end;
       by_tma = __all_sync(0xffffffffu, by_tma && slot[0] >= 0 && slot[kHalves - 1] >= 0);
       uint64_t* full = is_v ? &sh->v_full[st] : &sh->k_full[st];
@@ -522,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   } else if (warp == 12 && lane == 0) {
     // ================================ MMA issue ===========================================
     const uint32_t q_addr = smem_u32(s_q), k_base = smem_u32(s_k), v_base = smem_u32(s_v);
-    const int nt[2] = {nt0, nt1};
+    const int nt[2] = {nt0, nt1}, begin[2] = {head0, 0};
     bool alive = true;
     // Operand descriptors are built once; a k-step or a ring stage only moves the 14-bit address field (units of
     // 16 bytes) in the lower half, so the issue loop is one 32-bit add per operand and the MMA itself.
@@ -551,7 +674,43 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       }
       umma_commit(pv_bar(t, j));
     };
-    if (kTiles == 1) {
+    if (NARROW) {
+      // Two chains over alternating KV tiles, Q.K^T two tiles ahead of P.V: QK(0), QK(1), then PV(j), QK(j+2) per tile.
+      for (int a = 0; a < 2 && a < n_tiles && alive; ++a) {
+        alive = bar_wait(&sh->k_full[a], 0, &sh->abort);
+        if (!alive) break;
+        fence_async_smem();
+        tc_fence_after();
+        issue_qk(0, a, a);
+        umma_commit(&sh->k_free[a]);
+      }
+      int ks = 2, kround = 0, vs = 0, vround = 0;
+      for (int j = 0; j < n_tiles && alive; ++j) {
+        alive = bar_wait(&sh->v_full[vs], vround & 1, &sh->abort) &&
+                bar_wait(&sh->p_full[j & 1], (j >> 1) & 1, &sh->abort);
+        if (!alive) break;
+        fence_async_smem();
+        tc_fence_after();
+        issue_pv(j & 1, j & 1, j >> 1, vs);
+        umma_commit(&sh->v_free[vs]);
+        if (j + 2 < n_tiles) {                 // the buffer P.V(j) reads is free once that product has run: in order
+          alive = bar_wait(&sh->k_full[ks], kround & 1, &sh->abort);
+          if (!alive) break;
+          fence_async_smem();
+          tc_fence_after();
+          issue_qk(0, j & 1, ks);
+          umma_commit(&sh->k_free[ks]);
+          if (++ks == kKRing) {
+            ks = 0;
+            ++kround;
+          }
+        }
+        if (++vs == kVStages) {
+          vs = 0;
+          ++vround;
+        }
+      }
+    } else if (kTiles == 1) {
       // One query tile, two score buffers: Q.K^T runs two KV tiles ahead of P.V, so the tensor pipe has the next
       // tile's scores ready while this tile's softmax runs.  Order: QK(0), QK(1), then PV(j), QK(j+2) per tile.
       for (int a = 0; a < 2 && a < n_tiles && alive; ++a) {
@@ -592,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
         fence_async_smem();
         tc_fence_after();
         for (int t = 0; t < 2; ++t)
-          if (nt[t] > 0) issue_qk(t, t, 0);
+          if (nt[t] > 0 && begin[t] == 0) issue_qk(t, t, 0);
         umma_commit(&sh->k_free[0]);
       }
     }
@@ -605,13 +764,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       fence_async_smem();
       tc_fence_after();
       for (int t = 0; t < 2 && alive; ++t) {
-        if (j < nt[t]) {
-          alive = bar_wait(&sh->p_full[t], j & 1, &sh->abort);
+        const int mine = j - begin[t];                 // this query tile's own count
+        if (mine >= 0 && mine < nt[t]) {
+          alive = bar_wait(&sh->p_full[t], mine & 1, &sh->abort);
           if (!alive) break;
           tc_fence_after();
-          issue_pv(t, t, j, vs);
+          issue_pv(t, t, mine, vs);
         }
-        if (j + 1 < nt[t]) issue_qk(t, t, ks);
+        if (mine + 1 >= 0 && mine + 1 < nt[t]) issue_qk(t, t, ks);
       }
       if (!alive) break;
       umma_commit(&sh->v_free[vs]);
@@ -634,10 +794,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
 }
 
-template <int D, bool BIASED, bool SHARED>
+template <int D, bool BIASED, int FORM>
 int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream_t stream) {
   static std::atomic<bool> configured[64];
-  const int ready = opt_in_shared_memory(paged_prefill_tc_kernel<D, BIASED, SHARED>, Geo<D>::kSmemBytes, configured);
+  const int ready = opt_in_shared_memory(paged_prefill_tc_kernel<D, BIASED, FORM>, Geo<D>::kSmemBytes, configured);
   if (ready != GK_OK) return ready;
   {
     // Never launch if the register pool of this build cannot satisfy the budgets (the kernel would hang).
@@ -645,7 +805,7 @@ int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream
     int regs = launch_regs.load(std::memory_order_acquire);
     if (regs < 0) {
       cudaFuncAttributes attr;
-      if (cudaFuncGetAttributes(&attr, paged_prefill_tc_kernel<D, BIASED, SHARED>) != cudaSuccess) return check_launch();
+      if (cudaFuncGetAttributes(&attr, paged_prefill_tc_kernel<D, BIASED, FORM>) != cudaSuccess) return check_launch();
       regs = attr.numRegs;
       launch_regs.store(regs, std::memory_order_release);
     }
@@ -664,7 +824,11 @@ int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream
     p.tma_rows = box_rows;
   const int64_t ctas = n_work * p.kv_heads * (Geo<D>::kTiles == 2 ? 1 : 2);
   if (ctas > 0x7fffffffLL) return GK_ERR_UNSUPPORTED;
-  paged_prefill_tc_kernel<D, BIASED, SHARED><<<(unsigned)ctas, kThreads, Geo<D>::kSmemBytes, stream>>>(p, map_k, map_v);
+  if (FORM == kRowsForm)
+    paged_prefill_tc_kernel<D, BIASED, FORM><<<(unsigned)ctas, kThreads, Geo<D>::kSmemBytes, stream>>>(p, map_k, map_v);
+  else
+    launch_after_predecessor(paged_prefill_tc_kernel<D, BIASED, FORM>, dim3((unsigned)ctas), dim3(kThreads),
+                             Geo<D>::kSmemBytes, stream, p, map_k, map_v);
   return check_launch();
 }
 
@@ -675,15 +839,16 @@ struct PrefillExtras {
   const float* slopes = nullptr;
   const int32_t* row_limits = nullptr;
   const int32_t* list = nullptr;
+  bool narrow = false;
   float* part_ml = nullptr;
   float* part_o = nullptr;
 };
 
-template <bool BIASED, bool SHARED>
+template <bool BIASED, int FORM>
 int launch_prefill_dim(PrefillParams& p, int head_dim, int64_t n_work, int page_tokens, cudaStream_t stream) {
-  if (head_dim == 64) return launch_prefill<64, BIASED, SHARED>(p, n_work, page_tokens, stream);
-  if (head_dim == 256) return launch_prefill<256, BIASED, SHARED>(p, n_work, page_tokens, stream);
-  return launch_prefill<128, BIASED, SHARED>(p, n_work, page_tokens, stream);
+  if (head_dim == 64) return launch_prefill<64, BIASED, FORM>(p, n_work, page_tokens, stream);
+  if (head_dim == 256) return launch_prefill<256, BIASED, FORM == kNarrowForm ? kWideForm : FORM>(p, n_work, page_tokens, stream);
+  return launch_prefill<128, BIASED, FORM>(p, n_work, page_tokens, stream);
 }
 
 int prefill_entry(const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v, int64_t slots,
@@ -738,11 +903,14 @@ int prefill_entry(const void* q, int64_t q_row_stride, const void* pool_k, const
   p.part_ml = extras.part_ml;
   p.part_o = extras.part_o;
   cudaStream_t at = reinterpret_cast<cudaStream_t>(stream);
+  if (shared && extras.narrow)
+    return p.slopes ? launch_prefill_dim<true, kNarrowForm>(p, head_dim, n_work, page_tokens, at)
+                    : launch_prefill_dim<false, kNarrowForm>(p, head_dim, n_work, page_tokens, at);
   if (shared)
-    return p.slopes ? launch_prefill_dim<true, true>(p, head_dim, n_work, page_tokens, at)
-                    : launch_prefill_dim<false, true>(p, head_dim, n_work, page_tokens, at);
-  return p.slopes || p.row_limits ? launch_prefill_dim<true, false>(p, head_dim, n_work, page_tokens, at)
-                                  : launch_prefill_dim<false, false>(p, head_dim, n_work, page_tokens, at);
+    return p.slopes ? launch_prefill_dim<true, kWideForm>(p, head_dim, n_work, page_tokens, at)
+                    : launch_prefill_dim<false, kWideForm>(p, head_dim, n_work, page_tokens, at);
+  return p.slopes || p.row_limits ? launch_prefill_dim<true, kRowsForm>(p, head_dim, n_work, page_tokens, at)
+                                  : launch_prefill_dim<false, kRowsForm>(p, head_dim, n_work, page_tokens, at);
 }
 
 }  // namespace
@@ -779,9 +947,9 @@ extern "C" int gk_paged_prefill_tc_biased_multi_bf16(const void* q, int64_t q_ro
 extern "C" int gk_shared_prefix_attn_bf16(const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v,
                                           int64_t slots, const int32_t* table, int64_t table_stride,
                                           int64_t table_entry_stride, int page_tokens, const int32_t* table_rows,
-                                          const int32_t* prefix_work, int64_t n_prefix_work, const int32_t* prefix_rows,
-                                          float* part_ml, float* part_o, const float* slopes, float scale, float softcap,
-                                          int window, int q_heads, int kv_heads, int head_dim, int32_t* status,
+                                          const int32_t* prefix_work, int64_t n_prefix_work, int form,
+                                          const int32_t* prefix_rows, float* part_ml, float* part_o, const float* slopes,
+                                          float scale, float softcap, int window, int q_heads, int kv_heads, int head_dim, int32_t* status,
                                           gk_stream_t stream) {
   if (n_prefix_work == 0) return GK_OK;
   if (!prefix_rows || q_heads <= 0 || kv_heads <= 0 || q_heads / kv_heads > GK_MAX_PACKED_ROWS)
@@ -789,6 +957,7 @@ extern "C" int gk_shared_prefix_attn_bf16(const void* q, int64_t q_row_stride, c
   gk::PrefillExtras extras;
   extras.slopes = slopes;
   extras.list = prefix_rows;
+  extras.narrow = (form & GK_SHARED_ONE_TILE) != 0;
   extras.part_ml = part_ml;
   extras.part_o = part_o;
   return gk::prefill_entry(q, q_row_stride, pool_k, pool_v, slots, table, table_stride, table_entry_stride, page_tokens,

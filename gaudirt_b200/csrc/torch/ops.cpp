@@ -47,9 +47,9 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
                   head_dim == plan.head_dim,
               "GaudiRT attention: invalid scale, stream, or head dimension");
   TORCH_CHECK(plan.sliding_window == sliding_window, "GaudiRT attention: plan sliding_window mismatch");
-  for (const auto& input : {query, key, value})
-    TORCH_CHECK(input.is_cuda() && input.device() == device && input.scalar_type() == at::kBFloat16 &&
-                    input.dim() == 2 && input.size(0) == plan.rows,
+  for (const at::Tensor* input : {&query, &key, &value})
+    TORCH_CHECK(input->is_cuda() && input->device() == device && input->scalar_type() == at::kBFloat16 &&
+                    input->dim() == 2 && input->size(0) == plan.rows,
                 "GaudiRT attention: Q/K/V must be BF16 device matrices with matching rows");
   TORCH_CHECK(query.size(1) == plan.query_heads * head_dim && (!store || key.size(1) == plan.kv_heads * head_dim) &&
                   value.size(1) == key.size(1) && locations.dim() == 1 && locations.numel() == plan.rows &&
@@ -116,7 +116,7 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
     // attention kernel behind it.  It reads no row of this step, so the store may come after it.
     check_status(gk_shared_prefix_attn_bf16(q.data_ptr(), q.stride(0), key_pool.data_ptr(), value_pool.data_ptr(), plan.slots,
                                             plan.table.data_ptr<int32_t>(), plan.table_stride, plan.entry_stride,
-                                            plan.page_tokens, table_rows, words + plan.prefix_offset, plan.n_prefix,
+                                            plan.page_tokens, table_rows, words + plan.prefix_offset, plan.n_prefix, plan.shared_form,
                                             words + plan.prefix_rows_offset, plan.part_ml.data_ptr<float>(),
                                             plan.part_o.data_ptr<float>(), slopes, scale_f, softcap_f, (int)sliding_window,
                                             (int)plan.query_heads, (int)plan.kv_heads, (int)head_dim, status, s),
@@ -129,7 +129,7 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
                      value_pool.data_ptr(), plan.slots, plan.table.data_ptr<int32_t>(), plan.table_stride,
                      plan.entry_stride, plan.page_tokens, table_rows, words, plan.n_work, outs.data(), (int)outs.size(),
                      out_stride, plan.part_ml.data_ptr<float>(), plan.part_o.data_ptr<float>(), counters, slopes, row_limits,
-                     plan.n_prefix > 0 ? words + plan.parts_before_offset : nullptr, scale_f, softcap_f,
+                     plan.n_prefix > 0 ? words + plan.parts_before_offset : nullptr, plan.shared_form, scale_f, softcap_f,
                      (int)sliding_window, (int)plan.query_heads, (int)plan.kv_heads, (int)head_dim, status, s),
                  "paged attention");
   else if (fused_store)

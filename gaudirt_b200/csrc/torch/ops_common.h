@@ -79,6 +79,7 @@ struct AttentionPlan {
   int64_t n_prefill = 0, prefill_offset = 0;   // query tiles for the tensor-core prefill kernel
   int64_t n_prefix = 0, prefix_offset = 0;     // shared prefixes: records, listed rows, and per row the states in front
   int64_t prefix_rows_offset = 0, parts_before_offset = 0;
+  int shared_form = 0;                         // GK_SHARED_ONE_TILE, GK_SHARED_SHORT_TAILS
   int64_t row_limits_offset = -1;              // last key each row sees (two-way prefixes only)
   int page_tokens = 1;
   // Every sequence of the step is one query block of the decode kernel (no other CTA reads a new row):
@@ -504,7 +505,7 @@ class PagedMetadata : public torch::CustomClassHolder {
     // Multi-row sequences go to the tensor-core prefill kernel, the rest -- decode rows and very
     // short chunks -- to the split-KV decode kernel.  Short chunks of a group that is attended to together stay with
     // its decode rows; a longer one reads the prefix once per 256 packed rows as it is and takes no part in the group.
-    const int64_t min_saved = prefix_sharing_ > 0 ? 0 : kSharedPrefixMinSavedBytes;
+    const int64_t min_saved = prefix_sharing_ > 0 ? 0 : shared_prefix_min_saved_bytes(head_dim);
     const std::vector<char> together = short_group_members(query_heads, kv_heads, head_dim, min_saved);
     std::vector<int32_t> offered, offered_two_way, rest;
     for (int64_t i = 0; i < n_seq; ++i) {
@@ -543,10 +544,11 @@ class PagedMetadata : public torch::CustomClassHolder {
     }
     const int64_t n_groups = static_cast<int64_t>(shared_tokens_.size());
     int64_t n_work = 0, n_combine = 0, entries = 0, n_prefix = 0, n_prefix_rows = 0;
+    int form = 0;
     auto build = [&](int32_t* work, int32_t* combine, int32_t* prefix_work, int32_t* prefix_rows) {
       return gk_shared_prefix_plan_build(rest.data(), n_rest, rest_two_way.data(), rest_groups.data(), shared_tokens_.data(),
                                          n_groups, (int)query_heads, (int)kv_heads, (int)head_dim, window, sm_count,
-                                         split_tokens_, prefix_split_tokens_, min_saved, work, n_work, &n_work, combine,
+                                         split_tokens_, prefix_split_tokens_, min_saved, &form, work, n_work, &n_work, combine,
                                          n_combine, &n_combine, &entries, prefix_work, n_prefix, &n_prefix, prefix_rows,
                                          n_prefix_rows, &n_prefix_rows);
     };
@@ -618,6 +620,7 @@ class PagedMetadata : public torch::CustomClassHolder {
     plan->n_prefill = n_prefill;
     plan->prefill_offset = prefill_offset;
     plan->n_prefix = n_prefix;
+    plan->shared_form = form;
     plan->prefix_offset = prefix_offset;
     plan->prefix_rows_offset = prefix_rows_offset;
     plan->parts_before_offset = parts_before_offset;
@@ -673,8 +676,11 @@ class PagedMetadata : public torch::CustomClassHolder {
   }
   int split_tokens_ = 0, prefill_min_rows_ = 0, fused_combine_ = -1;
   bool last_plan_fused_ = false;       // whether the plan built last merges its splits inside the attention kernel
-  // Reading less than this again costs less than one more launch and the merge of the prefix's states.
-  static constexpr int64_t kSharedPrefixMinSavedBytes = int64_t{24} << 20;
+  // Reading less than this again costs less than one more launch and the merge of the prefix's states.  Measured over 2
+  // to 32 members, prefixes of 512 to 32768 and tails of 40 and 400 tokens: break-even at 59-101 MB of K/V at head_dim
+  // 128 (22.0 us apart against 19.5 us together at 101 MB, 12.5 against 15.3 at 65 MB), 50-63 MB at 64 (17.5 against 14.4
+  // at 63 MB) and 30-50 MB at 256 (33.1 against 27.7 at 50 MB).
+  static int64_t shared_prefix_min_saved_bytes(int64_t head_dim) { return (head_dim == 128 ? int64_t{80} : int64_t{48}) * 1000000; }
   int prefix_sharing_ = -1, prefix_split_tokens_ = 0;
   int64_t last_plan_prefix_records_ = 0;
   std::vector<int32_t> shared_groups_, shared_tokens_, two_way_;   // per sequence, per group, per sequence
@@ -691,11 +697,12 @@ class PagedMetadata : public torch::CustomClassHolder {
       in[i] = 1;
       ++members[static_cast<size_t>(shared_groups_[i])];
     }
+    int64_t saved = 0;
+    for (size_t g = 0; g < members.size(); ++g)
+      if (members[g] >= 2) saved += (members[g] - 1) * shared_tokens_[g] * kv_heads * head_dim * 4;
+    if (saved < min_saved) return {};
     for (size_t i = 0; i < in.size(); ++i)
-      if (in[i]) {
-        const int64_t count = members[static_cast<size_t>(shared_groups_[i])], tokens = shared_tokens_[static_cast<size_t>(shared_groups_[i])];
-        in[i] = count >= 2 && tokens > 0 && (count - 1) * tokens * kv_heads * head_dim * 4 >= min_saved;
-      }
+      if (in[i]) in[i] = members[static_cast<size_t>(shared_groups_[i])] >= 2 && shared_tokens_[static_cast<size_t>(shared_groups_[i])] > 0;
     return in;
   }
   // Compares the table rows of every group on the device; launches only.

@@ -3,6 +3,8 @@
 // Registered in ops.cpp.
 #include "ops_common.h"
 
+#include <ATen/cuda/EmptyTensor.h>
+
 namespace gaudirt_b200 {
 
 // ---------------------------------------------------------------------------------------------
@@ -106,14 +108,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
                   batch <= 65536 && mapping.size(0) <= 262144,
               "GaudiRT paged allocator: unsupported page size, row count or request count");
   c10::cuda::CUDAGuard guard(device);
-  const auto i32 = batch_requests.options(), i64 = lengths.options();
-  auto locations = at::empty({rows}, i32), positions = at::empty({rows}, i32), row_requests = at::empty({rows}, i32);
-  auto row_offsets = at::empty({batch + 1}, i32);
-  auto next_lengths = at::empty({batch}, i64), next_used = at::empty({1}, i64);
+  // straight from the caching allocator: six outputs through the dispatcher cost the host as much as the launch
+  auto vector = [&](int64_t n, at::ScalarType type) {
+    return at::Tensor(at::detail::empty_cuda({n}, type, device, c10::nullopt));
+  };
+  auto locations = vector(rows, at::kInt), positions = vector(rows, at::kInt), row_requests = vector(rows, at::kInt);
+  auto row_offsets = vector(batch + 1, at::kInt);
+  auto next_lengths = vector(batch, at::kLong), next_used = vector(1, at::kLong);
   uint64_t bytes = 0;
   check_status(gk_extend_requests_workspace_bytes(batch, &bytes), "paged allocator");
   at::Tensor workspace;
-  if (bytes > 0) workspace = at::empty({static_cast<int64_t>(bytes)}, i32.dtype(at::kByte));
+  if (bytes > 0) workspace = vector(static_cast<int64_t>(bytes), at::kByte);
   check_status(gk_extend_requests(mapping.data_ptr<int32_t>(), mapping.size(0), mapping.size(1), mapping.stride(0),
                                   batch_requests.data_ptr<int32_t>(), lengths.data_ptr<int64_t>(),
                                   new_tokens.data_ptr<int32_t>(), batch, free_pages.data_ptr<int64_t>(), free_pages.numel(),

@@ -21,11 +21,11 @@ def build(seq, groups, prefixes, q_heads, kv_heads, head_dim, window=-1, two_way
     as32 = lambda x: None if x is None else np.ascontiguousarray(x, dtype=np.int32)  # noqa: E731
     seq, groups, prefixes, two_way = as32(seq), as32(groups), as32(prefixes), as32(two_way)
     counts = [C.c_int64() for _ in range(5)]
-    refs = [C.byref(c) for c in counts]
+    refs, form = [C.byref(c) for c in counts], C.c_int()
 
     def call(work, combine, prefix, rows, caps):
         return lib.gk_shared_prefix_plan_build(ptr(seq), len(seq), ptr(two_way), ptr(groups), ptr(prefixes), len(prefixes),
-                                               q_heads, kv_heads, head_dim, window, sms, split, pieces, min_saved, ptr(work),
+                                               q_heads, kv_heads, head_dim, window, sms, split, pieces, min_saved, C.byref(form), ptr(work),
                                                caps[0], refs[0], ptr(combine), caps[1], refs[1], refs[2], ptr(prefix), caps[3],
                                                refs[3], ptr(rows), caps[4], refs[4])
 
@@ -39,6 +39,7 @@ def build(seq, groups, prefixes, q_heads, kv_heads, head_dim, window=-1, two_way
         return rc
     assert [c.value for c in counts] == n
     work, combine, prefix, rows = (a[:k] for a, k in zip(arrays, (n[0], n[1], n[3], n[4])))
+    assert not form.value & 1 or all(w[1] <= 128 // (q_heads // kv_heads) for w in prefix)
     return work, combine, n[2], prefix, rows
 
 
@@ -181,13 +182,13 @@ def test_launch_arguments_are_judged_on_the_host():
         args = list(check)
         args[at] = value
         assert lib.gk_shared_prefix_check(*args) == INVALID, at
-    attend = [one, 1024, one, one, 64, one, 16, 1, 1, None, one, 1, one, one, one, None, 1.0, 0.0, -1, 8, 2, 128, None, None]
-    for at, value in ((0, None), (10, None), (12, None), (13, None), (14, None), (12, C.c_void_p(4100)), (15, C.c_void_p(4097)),
-                      (16, 0.0), (17, -1.0), (18, 0), (8, 3)):
+    attend = [one, 1024, one, one, 64, one, 16, 1, 1, None, one, 1, 0, one, one, one, None, 1.0, 0.0, -1, 8, 2, 128, None, None]
+    for at, value in ((0, None), (10, None), (13, None), (14, None), (15, None), (13, C.c_void_p(4100)), (16, C.c_void_p(4097)),
+                      (17, 0.0), (18, -1.0), (19, 0), (8, 3)):
         args = list(attend)
         args[at] = value
         assert lib.gk_shared_prefix_attn_bf16(*args) == INVALID, at
-    for at, value in ((19, 34), (21, 96)):
+    for at, value in ((20, 34), (22, 96)):
         args = list(attend)
         args[at] = value
         assert lib.gk_shared_prefix_attn_bf16(*args) == UNSUPPORTED, at
