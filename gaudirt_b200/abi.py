@@ -45,8 +45,8 @@ PROTOTYPES = {
     "gk_shared_prefix_attn_bf16": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64, i32, vp, vp, vp, vp, f32, f32, i32,
                                          i32, i32, i32, vp, vp]),
     "gk_paged_attn_extended_multi_bf16": (i32, [vp, i64, vp, vp, i64, i64, vp, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64,
-                                                vp, i32, i64, vp, vp, vp, vp, vp, vp, i32, f32, f32, i32, i32, i32, i32, vp,
-                                                vp]),
+                                                vp, i64, vp, i32, i64, vp, vp, vp, vp, vp, i32, f32, f32, i32, i32, i32, i32,
+                                                vp, vp]),
     "gk_paged_prefill_tc_biased_multi_bf16": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, vp, i64, vp, i32, i64, vp,
                                                     vp, f32, f32, i32, i32, i32, i32, vp, vp]),
     "gk_peer_barrier": (i32, [vp, i32, i32, i32, i64, vp, vp]),

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <utility>
 
 #include "../../include/gaudirt_b200.h"
 
@@ -54,8 +55,8 @@ __device__ __forceinline__ void wait_for_predecessor() {
 }
 
 template <typename... Params, typename... Args>
-inline void launch_after_predecessor(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared_bytes,
-                                     cudaStream_t stream, Args&&... args) {
+inline void launch_programmatic(bool on, void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared_bytes,
+                                cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = block;
@@ -65,8 +66,15 @@ inline void launch_after_predecessor(void (*kernel)(Params...), dim3 grid, dim3 
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
-  config.numAttrs = g_programmatic_launch.load(std::memory_order_relaxed) ? 1 : 0;
+  config.numAttrs = on ? 1 : 0;
   (void)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);   // the caller reads the error with check_launch()
+}
+
+template <typename... Params, typename... Args>
+inline void launch_after_predecessor(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared_bytes,
+                                     cudaStream_t stream, Args&&... args) {
+  launch_programmatic(g_programmatic_launch.load(std::memory_order_relaxed) != 0, kernel, grid, block, shared_bytes, stream,
+                      std::forward<Args>(args)...);
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <array>
 #include <climits>
+#include <cmath>
 #include <functional>
 #include <cstdint>
 #include <numeric>
@@ -432,61 +433,81 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
     shared.push_back(&one);
   }
   if (saved < min_saved_bytes) shared.clear();
-  // Records of one query tile keep two chains of products going and wait less (0.98 us for a 128-row tile and 128 keys,
-  // 2.3 us for two tiles together), records of two fetch every key tile for twice as many rows.  Measured at head_dim 128:
-  // one tile 4-8 % faster at up to 14 tile products per SM, two tiles 2-6 % faster at 55 and 110.
-  int64_t most_rows = 0, products = 0;
-  for (const Group* g : shared) {
-    most_rows = std::max(most_rows, g->rows);
-    products += (g->rows + tile_rows - 1) / tile_rows * ((g->hi - g->lo + tile - 1) / tile) * kv_heads;
-  }
-  const bool one_tile = head_dim != 256 && !shared.empty() && (most_rows <= tile_rows || products < 32 * (int64_t)sm_count);
-  const int record_rows = one_tile ? tile_rows : GK_PREFILL_TILES_PER_ITEM * tile_rows;
-  // How long a piece of the prefix one CTA takes: the cheapest of the whole-tile lengths, by the time the CTAs need on
-  // sm_count SMs (one CTA each), in units of one key tile.  A CTA costs its tiles and a fixed prologue and
-  // epilogue; every piece leaves (m, l, O) states that are written and read once more.
+  // The form of the records (one or two query tiles) and how long a piece of the prefix one CTA takes: the cheapest by a
+  // model of the two kernels side by side, in us.  A prefix CTA has an SM to itself for a fixed 7 us and 1.2 us per 128 keys
+  // and one query tile, 2.4 us per two (1.0 and 1.9 at head_dim 64, 1.1 per 64 keys at 256).  The members' own CTAs take
+  // 3.5 us and 36 GB/s each; two per SM run on the SMs that the prefix leaves and on all of them once it is done.  Neither
+  // is faster than memory gives the bytes of both.  Every part of a row costs its merge 0.15 us.  So the longer of the two
+  // gets the SMs: measured with 256 members of 4096 + 1024 tokens, 32 CTAs of two tiles or 64 of one 108 us, 128 of one
+  // 123 us; with 32 members of 2048 + 256, 32 CTAs 16.7 us, 64 of them 18.4 us, 128 of them 23.7 us.
+  bool one_tile = head_dim != 256;
   int64_t piece = prefix_split_tokens;
-  if (piece == 0 && !shared.empty()) {
+  if (!shared.empty()) {
+    constexpr double kFixed = 7.0, kTailFixed = 3.5, kTailBytes = 36e3, kMemoryBytes = 5.9e6, kMergePart = 0.15;
+    const double one_time = head_dim == 64 ? 1.0 : head_dim == 128 ? 1.2 : 1.1, two_time = head_dim == 64 ? 1.9 : 2.4;
+    const double head_bytes = head_dim * 4.0;
+    double all_bytes = 0.0, tail_time = 0.0, tail_longest = 0.0;
+    int64_t tail_ctas = 0;
+    std::vector<int32_t> starts(static_cast<size_t>(n_seq), 0);
     int32_t longest = 0;
-    for (const Group* g : shared) longest = std::max(longest, g->hi - g->lo);
-    const double kCtaTiles = one_tile ? 7.0 : 3.0;                // 7-8 us
-    constexpr double kPartTiles = 0.15;                           // what one more part costs a row's merge
-    double best = 0.0;
-    for (int64_t tiles = 1; tiles <= (longest + tile - 1) / tile; tiles = tiles < 16 ? tiles + 1 : tiles + tiles / 8) {
-      std::vector<int32_t> costs;                                 // tiles per CTA; the scheduler takes them in order
-      int64_t most_parts = 0;
+    for (const Group* g : shared) {
+      for (int32_t s : g->members) starts[s] = g->hi;
+      longest = std::max(longest, g->hi - g->lo);
+      all_bytes += (double)(g->hi - g->lo) * kv_heads * head_bytes;
+    }
+    for (int64_t s = 0; s < n_seq; ++s) {
+      const int32_t* r = seq + s * 4;
+      const int64_t from = std::max<int64_t>(starts[s], window > 0 ? std::max(0, r[2] - window + 1) : 0);
+      const double bytes = (double)((int64_t)r[2] + r[1] - from) * head_bytes, time = kTailFixed + bytes / kTailBytes;
+      const int64_t ctas = (r[1] + GK_MAX_PACKED_ROWS / group_heads - 1) / (GK_MAX_PACKED_ROWS / group_heads) * kv_heads;
+      all_bytes += ctas * bytes;
+      tail_ctas += ctas;
+      tail_time += ctas * time;
+      tail_longest = std::max(tail_longest, time);
+    }
+    const double tail_mean = tail_time / (double)tail_ctas;
+    auto estimate = [&](bool one, int64_t tiles) {
+      int64_t ctas = 0, most_parts = 0;
+      double busy = 0.0, slowest = 0.0;
       for (const Group* g : shared) {
-        const int64_t records = (g->rows + record_rows - 1) / record_rows * kv_heads * ctas_per_record;
+        const int64_t rows_per_record = one ? tile_rows : GK_PREFILL_TILES_PER_ITEM * tile_rows;
+        const int64_t records = (g->rows + rows_per_record - 1) / rows_per_record * kv_heads * ctas_per_record;
         const int64_t span = (g->hi - g->lo + tile - 1) / tile, pieces = (span + tiles - 1) / tiles;
-        const int64_t even = (span + pieces - 1) / pieces;
+        const double per_tile = one || head_dim == 256 ? one_time : g->rows > tile_rows ? two_time : 1.8 * one_time;
+        ctas += records * pieces;
+        busy += records * (pieces * kFixed + span * per_tile);
+        slowest = std::max(slowest, kFixed + (double)((span + pieces - 1) / pieces) * per_tile);
         most_parts = std::max(most_parts, pieces);
-        if (pieces * records > 16 * (int64_t)sm_count) { costs.clear(); break; }
-        for (int64_t i = 0; i < pieces; ++i)
-          for (int64_t k = 0; k < records; ++k) costs.push_back((int32_t)std::min<int64_t>(even, span - i * even));
       }
-      if (costs.empty()) {
-        if (tiles < (longest + tile - 1) / tile) continue;
-        piece = tiles * tile;                                     // many CTAs whatever the cut: no cut at all
-        break;
+      const double waves = (double)((ctas + sm_count - 1) / sm_count);
+      const double prefix = std::max(slowest, waves > 1.0 ? waves * busy / (double)ctas : 0.0);
+      const double slots = 2.0 * (double)std::max<int64_t>(0, sm_count - ctas);
+      double tails = tail_longest;
+      if ((double)tail_ctas > slots) {
+        const double left = std::max(0.0, (double)tail_ctas - std::floor(prefix / tail_mean) * slots);
+        tails = left > 0.0 ? prefix + std::max(1.0, left / (2.0 * sm_count)) * tail_mean : prefix;
       }
-      std::sort(costs.begin(), costs.end(), std::greater<int32_t>());
-      std::vector<double> heap((size_t)sm_count, 0.0);
-      auto later = std::greater<double>();
-      double makespan = 0.0;
-      for (int32_t c : costs) {
-        std::pop_heap(heap.begin(), heap.end(), later);
-        heap.back() += c + kCtaTiles;
-        makespan = std::max(makespan, heap.back());
-        std::push_heap(heap.begin(), heap.end(), later);
-      }
-      const double cost = makespan + kPartTiles * (double)most_parts;
-      if (piece == 0 || cost < best) {
+      return std::max({prefix, tails, all_bytes / kMemoryBytes}) + kMergePart * (double)most_parts;
+    };
+    double best = -1.0;
+    const int64_t all_tiles = (longest + tile - 1) / tile, given = (piece + tile - 1) / tile;
+    std::vector<int64_t> lengths;                                 // of a piece, in tiles: every one up to 16, then in steps of an eighth
+    if (given > 0) lengths.push_back(given);
+    for (int64_t tiles = 1; given == 0 && tiles < all_tiles; tiles += std::max<int64_t>(1, tiles < 16 ? 1 : tiles / 8)) lengths.push_back(tiles);
+    if (given == 0) lengths.push_back(all_tiles);
+    for (bool one : {true, false}) {
+      if (one && head_dim == 256) continue;
+      for (const int64_t tiles : lengths) {
+        const double cost = estimate(one, tiles);
+        if (best >= 0.0 && cost >= best) continue;
         best = cost;
-        piece = tiles * tile;
+        one_tile = one;
+        if (given == 0) piece = tiles * tile;
       }
     }
+    piece = round_up(std::max<int64_t>(piece, tile), tile);
   }
-  if (piece > 0) piece = round_up(std::max<int64_t>(piece, tile), tile);
+  const int record_rows = one_tile ? tile_rows : GK_PREFILL_TILES_PER_ITEM * tile_rows;
 
   std::vector<int32_t> kv_from(static_cast<size_t>(n_seq), 0), before(static_cast<size_t>(n_seq), 0);
   struct Item { int32_t w[GK_WORK_WORDS]; };
@@ -529,7 +550,7 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
   for (int64_t s = 0; s < n_seq; ++s) own_tokens += seq[s * 4 + 2] + seq[s * 4 + 1] - kv_from[s];
   const bool short_tails = head_dim != 256 && !items.empty() && *n_work_out * kv_heads >= 6 * (int64_t)sm_count &&
                            own_tokens <= 2048 * *n_work_out;
-  *form_out = (one_tile ? GK_SHARED_ONE_TILE : 0) | (short_tails ? GK_SHARED_SHORT_TAILS : 0);
+  *form_out = items.empty() ? 0 : GK_SHARED_PREFIX | (one_tile ? GK_SHARED_ONE_TILE : 0) | (short_tails ? GK_SHARED_SHORT_TAILS : 0);
   *n_prefix_work_out = (int64_t)items.size();
   *n_prefix_rows_out = (int64_t)rows.size();
   if (!work_out) return GK_OK;

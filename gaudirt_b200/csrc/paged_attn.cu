@@ -59,7 +59,7 @@ struct AttnParams {
   // read by the extended form only (template argument EXT), each may be null:
   const float* slopes;                   // [q_heads]: the score of key j gets -slope * |position - j|
   const int32_t* row_limits;             // [rows]: last key a row sees, at or behind its position (two-way prefix)
-  const int32_t* parts_before;           // [rows]: states of a shared prefix that stand in front of the block's own splits
+  bool beside;                           // runs beside the shared-prefix kernel in front of it (see the kernel's first lines)
 };
 
 template <int D, int WARPS, int STAGES>
@@ -84,15 +84,18 @@ __device__ __forceinline__ uint32_t group_off(int row, int chunk) {
   return (chunk >> 3) * (kGroupTokens * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
-// EXT: distance bias, row limits and states of a shared prefix; without it none of the three costs an instruction.
+// EXT: distance bias, row limits and the launch beside a shared-prefix kernel; without it none of the three costs an
+// instruction.
 template <int D, int WARPS, int STAGES, bool TMA, bool EXT>
 __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const AttnParams p,
                                                                    const __grid_constant__ CUtensorMap map_kv) {
   using C = AttnConfig<D, WARPS, STAGES>;
   extern __shared__ __align__(1024) uint8_t smem[];     // swizzle atoms of the TMA boxes are 1 KiB
   // Behind a shared prefix the kernel before this one is the prefix's, which released this one after everything before it
-  // had completed: only the merge has to wait for it, the rest runs beside it.
-  if (EXT && p.parts_before)
+  // had completed.  The two have nothing to do with each other -- this kernel leaves states for the combine launch behind
+  // it -- so nothing waits here; only the last CTA does, at its very end, so that this launch is not complete before the
+  // prefix's is.
+  if (EXT && p.beside)
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   else
     wait_for_predecessor();
@@ -107,8 +110,6 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const
   const int n_splits = w1.w & 0xffff, split_index = (w1.w >> 16) & 0x7fff;
   const int G = p.group;
   const int mv = n_rows * G;                                    // packed rows in use (<= 16)
-  // states of a shared prefix in front of this block's own (their kernel ran before this one)
-  const int before = EXT && p.parts_before ? __ldg(p.parts_before + first_row) : 0;
 
   // ---- Q fragments (A operand of S = Q K^T), rows g and g+8 of the packed tile ----------
   uint32_t qf[D / 16][4];
@@ -450,7 +451,6 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const
     }
   }
   __syncthreads();
-  if (EXT && p.parts_before) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
   for (int idx = threadIdx.x; idx < mv * (D / 4); idx += WARPS * 32) {
     const int prow = idx / (D / 4), c4 = idx - prow * (D / 4);
@@ -478,47 +478,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const
       }
     }
     const int r = prow / G, gq = prow - r * G;
-    if (EXT && before > 0 && n_splits == before + 1) {
-      // The whole of the block's own range is here: fold the prefix's states in, four at a time (their loads are
-      // independent), and write the row.
-      const int stride = n_rows * p.q_heads;
-      const int64_t e0 = (int64_t)partial_base - (int64_t)before * stride + (int64_t)r * p.q_heads + head * G + gq;
-      if (e0 < 0 || (int64_t)partial_base + (int64_t)r * p.q_heads + head * G + gq >= p.part_capacity) {
-        if (c4 == 0 && p.status) atomicOr(p.status, (int)GK_DEV_BAD_SLOT);
-        continue;
-      }
-      for (int s0 = 0; s0 < before; s0 += 4) {
-        float2 ml[4];
-        float4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t entry = e0 + (int64_t)min(s0 + i, before - 1) * stride;
-          ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + entry);
-          v[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + entry * D) + c4);
-          if (s0 + i >= before) ml[i].y = 0.f;
-        }
-        float top = mstar;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = ml[i].y > 0.f ? fmaxf(top, ml[i].x) : top;
-        const float keep = lsum > 0.f ? fast_exp2(mstar - top) : 0.f;
-        mstar = top;
-        lsum *= keep;
-        acc.x *= keep;
-        acc.y *= keep;
-        acc.z *= keep;
-        acc.w *= keep;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float wgt = ml[i].y > 0.f ? fast_exp2(ml[i].x - top) : 0.f;
-          lsum += wgt * ml[i].y;
-          acc.x += wgt * v[i].x;
-          acc.y += wgt * v[i].y;
-          acc.z += wgt * v[i].z;
-          acc.w += wgt * v[i].w;
-        }
-      }
-    }
-    if (partial_base < 0 || (EXT && before > 0 && n_splits == before + 1)) {
+    if (partial_base < 0) {
       const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
       uint2 packed;
       packed.x = pack_bf16(acc.x * inv, acc.y * inv);
@@ -539,14 +499,14 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const
   // ---- fused combine: the CTA that completes a block's last split merges all of them ---------
   // Arrival order decides only WHO merges; the merge itself runs over the splits in split order, so
   // the result does not depend on scheduling.  The counter returns to zero for the next launch.
-  if (partial_base >= 0 && p.counters != nullptr && !(EXT && before > 0 && n_splits == before + 1)) {
+  if (partial_base >= 0 && p.counters != nullptr) {
     __shared__ int is_last;
     __threadfence();                                   // this CTA's split state before its arrival
     __syncthreads();
     if (threadIdx.x == 0) {
       int* counter = p.counters + (int64_t)first_row * p.kv_heads + head;
       const int seen = atomicAdd(counter, 1);
-      is_last = seen == n_splits - before - 1;
+      is_last = seen == n_splits - 1;
       if (is_last) *counter = 0;
     }
     __syncthreads();
@@ -587,6 +547,7 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const
       }
     }
   }
+  if (EXT && p.beside && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 struct OutputList {
@@ -684,7 +645,8 @@ int launch_attn_form(const AttnParams& p, const CUtensorMap& map_kv, int64_t n_w
   const int ready = opt_in_shared_memory(kernel, C::kSmemBytes, configured);
   if (ready != GK_OK) return ready;
   const int64_t blocks = n_work * p.kv_heads;
-  launch_after_predecessor(kernel, dim3((unsigned)blocks), dim3(WARPS * 32), C::kSmemBytes, stream, p, map_kv);
+  launch_programmatic(p.beside || g_programmatic_launch.load(std::memory_order_relaxed) != 0, kernel, dim3((unsigned)blocks),
+                      dim3(WARPS * 32), C::kSmemBytes, stream, p, map_kv);
   return check_launch();
 }
 
@@ -719,11 +681,11 @@ int launch_attn(const AttnParams& p, int64_t n_work, int page_tokens, bool short
   const bool boxed = boxes && page_tokens >= kGroupTokens && pool_rows < 0x7fffffffLL &&
                      make_kv_group_map(&map_kv, p.pool_k, v_minus_k, pool_rows, kGroupTokens, D);
   if constexpr (D <= 128) {
-    if (short_tails && p.parts_before)
+    if (short_tails)
       return boxed ? launch_attn_form<D, true, true, 2>(p, map_kv, n_work, stream)
                    : launch_attn_form<D, false, true, 2>(p, map_kv, n_work, stream);
   }
-  if (p.slopes || p.row_limits || p.parts_before)
+  if (p.slopes || p.row_limits || p.beside)
     return boxed ? launch_attn_form<D, true, true>(p, map_kv, n_work, stream)
                  : launch_attn_form<D, false, true>(p, map_kv, n_work, stream);
   return boxed ? launch_attn_form<D, true, false>(p, map_kv, n_work, stream)
@@ -739,10 +701,11 @@ int attn_entry(const void* q, int64_t q_row_stride, const void* pool_k, const vo
                float scale, float softcap, int window, int q_heads, int kv_heads, int head_dim, int32_t* status,
                gk_stream_t stream, const void* new_k = nullptr, const void* new_v = nullptr, int64_t new_k_stride = 0,
                int64_t new_v_stride = 0, const int32_t* locations = nullptr, const float* slopes = nullptr,
-               const int32_t* row_limits = nullptr, const int32_t* parts_before = nullptr, int form = 0) {
+               const int32_t* row_limits = nullptr, int form = 0) {
   if (n_work == 0) return GK_OK;
-  if ((reinterpret_cast<uintptr_t>(slopes) | reinterpret_cast<uintptr_t>(row_limits) |
-       reinterpret_cast<uintptr_t>(parts_before)) & 3)
+  if (((reinterpret_cast<uintptr_t>(slopes) | reinterpret_cast<uintptr_t>(row_limits)) & 3) ||
+      (form & ~(GK_SHARED_ONE_TILE | GK_SHARED_SHORT_TAILS | GK_SHARED_PREFIX)) ||
+      ((form & GK_SHARED_PREFIX) && split_counters))
     return GK_ERR_INVALID_ARGUMENT;
   if (new_k || new_v || locations) {
     // the fused store moves whole 16-byte pieces
@@ -803,7 +766,7 @@ int attn_entry(const void* q, int64_t q_row_stride, const void* pool_k, const vo
   p.group = q_heads / kv_heads;
   p.slopes = slopes;
   p.row_limits = row_limits;
-  p.parts_before = parts_before;
+  p.beside = (form & GK_SHARED_PREFIX) != 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (head_dim) {
     case 64: return launch_attn<64>(p, n_work, page_tokens, form & GK_SHARED_SHORT_TAILS, s);
@@ -843,19 +806,6 @@ extern "C" int gk_paged_attn_store_multi_bf16(const void* q, int64_t q_row_strid
                         new_k_row_stride, new_v_row_stride, locations);
 }
 
-extern "C" int gk_paged_attn_extended_multi_bf16(
-    const void* q, int64_t q_row_stride, const void* new_k, const void* new_v, int64_t new_k_row_stride,
-    int64_t new_v_row_stride, const int32_t* locations, void* pool_k, void* pool_v, int64_t slots, const int32_t* table,
-    int64_t table_stride, int64_t table_entry_stride, int page_tokens, const int32_t* table_rows, const int32_t* work,
-    int64_t n_work, void* const* outs, int n_outs, int64_t out_row_stride, float* part_ml, float* part_o,
-    int32_t* split_counters, const float* slopes, const int32_t* row_limits, const int32_t* parts_before, int form,
-    float scale, float softcap, int window, int q_heads, int kv_heads, int head_dim, int32_t* status, gk_stream_t stream) {
-  return gk::attn_entry(q, q_row_stride, pool_k, pool_v, slots, table, table_stride, table_entry_stride, page_tokens,
-                        table_rows, work, n_work, outs, n_outs, out_row_stride, part_ml, part_o, INT64_MAX,
-                        split_counters, scale, softcap, window, q_heads, kv_heads, head_dim, status, stream, new_k, new_v,
-                        new_k_row_stride, new_v_row_stride, locations, slopes, row_limits, parts_before, form);
-}
-
 extern "C" int gk_paged_attn_bf16(const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v,
                                   int64_t slots, const int32_t* table, int64_t table_stride,
                                   int64_t table_entry_stride, int page_tokens, const int32_t* table_rows,
@@ -888,7 +838,7 @@ int combine_check(const float* part_ml, const float* part_o, const int32_t* comb
 
 int combine_entry(const float* part_ml, const float* part_o, int64_t capacity, const int32_t* combine,
                   int64_t n_combine, void* const* outs, int n_outs, int64_t out_row_stride, int q_heads, int head_dim,
-                  int32_t* status, gk_stream_t stream) {
+                  int32_t* status, gk_stream_t stream, bool behind_shared = false) {
   if (n_combine == 0) return GK_OK;
   const int checked = combine_check(part_ml, part_o, combine, n_combine, outs, n_outs, out_row_stride, q_heads, head_dim);
   if (checked != GK_OK) return checked;
@@ -899,15 +849,36 @@ int combine_entry(const float* part_ml, const float* part_o, int64_t capacity, c
   // Four entries per CTA; a decode record (one row) is covered in one pass, records with more
   // rows loop over them.
   const dim3 grid((unsigned)n_combine, (unsigned)((q_heads + 3) / 4));
+  const bool programmatic = behind_shared || g_programmatic_launch.load(std::memory_order_relaxed) != 0;
   switch (head_dim) {
-    case 64: launch_after_predecessor(paged_attn_combine_kernel<64>, grid, dim3(128), 0, s, part_ml, part_o, combine, o, out_row_stride, q_heads, capacity, status); break;
-    case 128: launch_after_predecessor(paged_attn_combine_kernel<128>, grid, dim3(128), 0, s, part_ml, part_o, combine, o, out_row_stride, q_heads, capacity, status); break;
-    default: launch_after_predecessor(paged_attn_combine_kernel<256>, grid, dim3(128), 0, s, part_ml, part_o, combine, o, out_row_stride, q_heads, capacity, status); break;
+    case 64: launch_programmatic(programmatic, paged_attn_combine_kernel<64>, grid, dim3(128), 0, s, part_ml, part_o, combine, o, out_row_stride, q_heads, capacity, status); break;
+    case 128: launch_programmatic(programmatic, paged_attn_combine_kernel<128>, grid, dim3(128), 0, s, part_ml, part_o, combine, o, out_row_stride, q_heads, capacity, status); break;
+    default: launch_programmatic(programmatic, paged_attn_combine_kernel<256>, grid, dim3(128), 0, s, part_ml, part_o, combine, o, out_row_stride, q_heads, capacity, status); break;
   }
   return check_launch();
 }
 }  // namespace
 }  // namespace gk
+
+extern "C" int gk_paged_attn_extended_multi_bf16(
+    const void* q, int64_t q_row_stride, const void* new_k, const void* new_v, int64_t new_k_row_stride,
+    int64_t new_v_row_stride, const int32_t* locations, void* pool_k, void* pool_v, int64_t slots, const int32_t* table,
+    int64_t table_stride, int64_t table_entry_stride, int page_tokens, const int32_t* table_rows, const int32_t* work,
+    int64_t n_work, const int32_t* combine, int64_t n_combine, void* const* outs, int n_outs, int64_t out_row_stride,
+    float* part_ml, float* part_o, int32_t* split_counters, const float* slopes, const int32_t* row_limits, int form,
+    float scale, float softcap, int window, int q_heads, int kv_heads, int head_dim, int32_t* status, gk_stream_t stream) {
+  if (n_combine < 0 || (split_counters && n_combine > 0)) return GK_ERR_INVALID_ARGUMENT;
+  if (n_work == 0) return n_combine == 0 ? GK_OK : GK_ERR_INVALID_ARGUMENT;
+  const int checked = gk::combine_check(part_ml, part_o, combine, n_combine, outs, n_outs, out_row_stride, q_heads, head_dim);
+  if (checked != GK_OK) return checked;
+  const int rc = gk::attn_entry(q, q_row_stride, pool_k, pool_v, slots, table, table_stride, table_entry_stride, page_tokens,
+                                table_rows, work, n_work, outs, n_outs, out_row_stride, part_ml, part_o, INT64_MAX,
+                                split_counters, scale, softcap, window, q_heads, kv_heads, head_dim, status, stream, new_k,
+                                new_v, new_k_row_stride, new_v_row_stride, locations, slopes, row_limits, form);
+  if (rc != GK_OK) return rc;
+  return gk::combine_entry(part_ml, part_o, INT64_MAX, combine, n_combine, outs, n_outs, out_row_stride, q_heads, head_dim,
+                           nullptr, stream, (form & GK_SHARED_PREFIX) != 0);
+}
 
 extern "C" int gk_paged_attn_combine_multi_bf16(const float* part_ml, const float* part_o, const int32_t* combine,
                                                 int64_t n_combine, void* const* outs, int n_outs,

@@ -827,8 +827,8 @@ int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream
   if (FORM == kRowsForm)
     paged_prefill_tc_kernel<D, BIASED, FORM><<<(unsigned)ctas, kThreads, Geo<D>::kSmemBytes, stream>>>(p, map_k, map_v);
   else
-    launch_after_predecessor(paged_prefill_tc_kernel<D, BIASED, FORM>, dim3((unsigned)ctas), dim3(kThreads),
-                             Geo<D>::kSmemBytes, stream, p, map_k, map_v);
+    launch_programmatic(true, paged_prefill_tc_kernel<D, BIASED, FORM>, dim3((unsigned)ctas), dim3(kThreads),
+                        Geo<D>::kSmemBytes, stream, p, map_k, map_v);
   return check_launch();
 }
 

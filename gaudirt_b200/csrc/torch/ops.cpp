@@ -112,8 +112,8 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
                                              value_pool.data_ptr(), plan.slots, (int)plan.kv_heads, (int)head_dim, status, s),
                  "KV store");
   if (plan.n_prefix > 0)
-    // The keys that several sequences share, once for all of their rows; the states it leaves are merged by the
-    // attention kernel behind it.  It reads no row of this step, so the store may come after it.
+    // The keys that several sequences share, once for all of their rows; the combine behind the attention kernel merges
+    // the states it leaves.  It reads no row of this step, so the store may come after it.
     check_status(gk_shared_prefix_attn_bf16(q.data_ptr(), q.stride(0), key_pool.data_ptr(), value_pool.data_ptr(), plan.slots,
                                             plan.table.data_ptr<int32_t>(), plan.table_stride, plan.entry_stride,
                                             plan.page_tokens, table_rows, words + plan.prefix_offset, plan.n_prefix, plan.shared_form,
@@ -122,15 +122,16 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
                                             (int)plan.query_heads, (int)plan.kv_heads, (int)head_dim, status, s),
                  "shared prefix attention");
   const int32_t* row_limits = plan.row_limits_offset >= 0 ? words + plan.row_limits_offset : nullptr;
-  if (slopes || row_limits || plan.n_prefix > 0)
+  const bool extended = slopes || row_limits || plan.n_prefix > 0;      // its call includes the combine launch
+  if (extended)
     check_status(gk_paged_attn_extended_multi_bf16(
                      q.data_ptr(), q.stride(0), fused_store ? k.data_ptr() : nullptr, fused_store ? v.data_ptr() : nullptr,
                      k.stride(0), v.stride(0), fused_store ? locations.data_ptr<int32_t>() : nullptr, key_pool.data_ptr(),
                      value_pool.data_ptr(), plan.slots, plan.table.data_ptr<int32_t>(), plan.table_stride,
-                     plan.entry_stride, plan.page_tokens, table_rows, words, plan.n_work, outs.data(), (int)outs.size(),
-                     out_stride, plan.part_ml.data_ptr<float>(), plan.part_o.data_ptr<float>(), counters, slopes, row_limits,
-                     plan.n_prefix > 0 ? words + plan.parts_before_offset : nullptr, plan.shared_form, scale_f, softcap_f,
-                     (int)sliding_window, (int)plan.query_heads, (int)plan.kv_heads, (int)head_dim, status, s),
+                     plan.entry_stride, plan.page_tokens, table_rows, words, plan.n_work, words + plan.combine_offset,
+                     counters ? 0 : plan.n_combine, outs.data(), (int)outs.size(), out_stride,
+                     plan.part_ml.data_ptr<float>(), plan.part_o.data_ptr<float>(), counters, slopes, row_limits,
+                     plan.shared_form, scale_f, softcap_f, (int)sliding_window, (int)plan.query_heads, (int)plan.kv_heads, (int)head_dim, status, s),
                  "paged attention");
   else if (fused_store)
     check_status(gk_paged_attn_store_multi_bf16(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), k.stride(0),
@@ -150,7 +151,7 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
                                           scale_f, softcap_f, (int)sliding_window, (int)plan.query_heads,
                                           (int)plan.kv_heads, (int)head_dim, status, s),
                  "paged attention");
-  if (!plan.counters.defined())     // otherwise the combine ran inside: the last split to finish merged its block
+  if (!extended && !plan.counters.defined())     // otherwise the combine ran inside: the last split to finish merged its block
     check_status(gk_paged_attn_combine_multi_bf16(plan.part_ml.data_ptr<float>(), plan.part_o.data_ptr<float>(),
                                                   words + plan.combine_offset, plan.n_combine, outs.data(),
                                                   (int)outs.size(), out_stride, (int)plan.query_heads, (int)head_dim, s),

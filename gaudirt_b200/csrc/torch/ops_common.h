@@ -77,9 +77,8 @@ struct AttentionPlan {
   int64_t rows = 0, slots = 0, query_heads = 0, kv_heads = 0, head_dim = 0, sliding_window = -1;
   int64_t n_work = 0, n_combine = 0, combine_offset = 0, table_stride = 0, entry_stride = 1;
   int64_t n_prefill = 0, prefill_offset = 0;   // query tiles for the tensor-core prefill kernel
-  int64_t n_prefix = 0, prefix_offset = 0;     // shared prefixes: records, listed rows, and per row the states in front
-  int64_t prefix_rows_offset = 0, parts_before_offset = 0;
-  int shared_form = 0;                         // GK_SHARED_ONE_TILE, GK_SHARED_SHORT_TAILS
+  int64_t n_prefix = 0, prefix_offset = 0, prefix_rows_offset = 0;     // shared prefixes: records and listed rows
+  int shared_form = 0;                         // GK_SHARED_* bits
   int64_t row_limits_offset = -1;              // last key each row sees (two-way prefixes only)
   int page_tokens = 1;
   // Every sequence of the step is one query block of the decode kernel (no other CTA reads a new row):
@@ -557,25 +556,13 @@ class PagedMetadata : public torch::CustomClassHolder {
     const int64_t prefill_offset = combine_offset + n_combine * GK_COMBINE_WORDS;
     const int64_t prefix_offset = prefill_offset + n_prefill * GK_WORK_WORDS;
     const int64_t prefix_rows_offset = prefix_offset + n_prefix * GK_WORK_WORDS;
-    const int64_t parts_before_offset = prefix_rows_offset + n_prefix_rows * 4;
-    const int64_t row_limits_offset = parts_before_offset + (n_prefix > 0 ? rows_ : 0);
+    const int64_t row_limits_offset = prefix_rows_offset + n_prefix_rows * 4;
     const int64_t words = std::max<int64_t>(4, row_limits_offset + (two_way_.empty() ? 0 : rows_));
     auto staging = at::empty({words}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
     int32_t* host = staging.data_ptr<int32_t>();
     if (n_rest > 0)
       check_status(build(host, host + combine_offset, host + prefix_offset, host + prefix_rows_offset), "attention plan");
     if (n_prefill > 0) check_status(build_prefill(host + prefill_offset), "prefill plan");
-    if (n_prefix > 0) {
-      int32_t* before = host + parts_before_offset;
-      std::fill(before, before + rows_, 0);
-      for (int64_t i = 0; i < n_prefix; ++i) {               // parts of a row: one more than its highest part index
-        const int32_t* w = host + prefix_offset + i * GK_WORK_WORDS;
-        for (int32_t r = 0; r < w[1]; ++r) {
-          int32_t& parts = before[host[prefix_rows_offset + ((int64_t)w[0] + r) * 4]];
-          parts = std::max(parts, w[2] + 1);
-        }
-      }
-    }
     if (!two_way_.empty()) {
       int32_t* limit = host + row_limits_offset;
       for (int64_t i = 0; i < n_seq; ++i)
@@ -596,8 +583,9 @@ class PagedMetadata : public torch::CustomClassHolder {
     // that the fused form costs nothing even with hundreds of them, and it saves the launch.
     int32_t most_splits = 0;
     for (int64_t i = 0; i < n_combine; ++i) most_splits = std::max(most_splits, host[combine_offset + i * GK_COMBINE_WORDS + 3]);
-    // Behind a shared prefix the merge is always part of the attention kernel: its splits follow the prefix's states.
-    const bool fuse = n_prefix > 0 || fused_combine_ > 0 || (fused_combine_ < 0 && (n_combine * 5 <= sm_count * 2 || most_splits <= 2));
+    // Behind a shared prefix the merge is always the combine kernel's: the attention kernel runs beside the prefix's and
+    // does not know its states.
+    const bool fuse = n_prefix == 0 && (fused_combine_ > 0 || (fused_combine_ < 0 && (n_combine * 5 <= sm_count * 2 || most_splits <= 2)));
     last_plan_fused_ = n_combine > 0 && fuse;
     if (n_combine > 0 && fuse)
       plan->counters = at::zeros({rows_ * kv_heads}, at::TensorOptions().dtype(at::kInt).device(device));
@@ -623,7 +611,6 @@ class PagedMetadata : public torch::CustomClassHolder {
     plan->shared_form = form;
     plan->prefix_offset = prefix_offset;
     plan->prefix_rows_offset = prefix_rows_offset;
-    plan->parts_before_offset = parts_before_offset;
     plan->row_limits_offset = two_way_.empty() ? -1 : row_limits_offset;
     last_plan_prefix_records_ = n_prefix;
     {

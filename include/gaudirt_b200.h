@@ -219,14 +219,15 @@ GK_API int gk_paged_prefill_tc_bf16(const void* q, int64_t q_row_stride, const v
  * gk_prefill_plan_build_two_way take two_way[n_seq], the number of leading tokens of each sequence that
  * all of its rows see (0 = causal; at most the sequence's last position + 1, so that every such key is
  * in the pool), for which row_limits[row] = max(position, two_way - 1).
- * parts_before, form: see the shared prefix below; NULL and 0 = none. */
+ * combine, n_combine: the plan's combine records, merged by a second launch of this call; 0 records
+ * with split_counters.  form: GK_SHARED_* bits of a plan with shared prefixes (below), 0 = none. */
 GK_API int gk_paged_attn_extended_multi_bf16(
     const void* q, int64_t q_row_stride, const void* new_k, const void* new_v, int64_t new_k_row_stride,
     int64_t new_v_row_stride, const int32_t* locations, void* pool_k, void* pool_v, int64_t slots,
     const int32_t* table, int64_t table_stride, int64_t table_entry_stride, int page_tokens,
-    const int32_t* table_rows, const int32_t* work, int64_t n_work, void* const* outs, int n_outs,
-    int64_t out_row_stride, float* part_ml, float* part_o, int32_t* split_counters, const float* slopes,
-    const int32_t* row_limits, const int32_t* parts_before, int form, float scale, float softcap,
+    const int32_t* table_rows, const int32_t* work, int64_t n_work, const int32_t* combine,
+    int64_t n_combine, void* const* outs, int n_outs, int64_t out_row_stride, float* part_ml,
+    float* part_o, int32_t* split_counters, const float* slopes, const int32_t* row_limits, int form, float scale, float softcap,
     int window, int q_heads, int kv_heads, int head_dim, int32_t* status, gk_stream_t stream);
 GK_API int gk_paged_prefill_tc_biased_multi_bf16(
     const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v, int64_t slots,
@@ -243,8 +244,8 @@ GK_API int gk_prefill_plan_build_two_way(const int32_t* seq, int64_t n_seq, cons
  * No counterpart in the reference.  Sequences of one group hold the same slots in their first
  * prefix_tokens[group] positions (a common system prompt, several samples of one prompt).  The plan
  * cuts every member's own work at the end of the prefix and adds records that attend to the prefix
- * once for all rows of the group; their states (m, l, O) are merged with the members' own by the
- * attention kernel, in a fixed order.
+ * once for all rows of the group; the combine launch merges their states (m, l, O) with the members'
+ * own, in a fixed order.
  *   seq, two_way  as above (two_way may be NULL); groups[n_seq]: group of each sequence or -1;
  *                 every member's first position lies at or behind the end of its group's prefix.
  *   min_saved_bytes   groups are attended to together when that saves at least so much reading in all.
@@ -252,8 +253,8 @@ GK_API int gk_prefill_plan_build_two_way(const int32_t* seq, int64_t n_seq, cons
  *                 at most one query tile of rows (n_rows <= GK_PREFILL_TILE_ROWS / group);
  *                 GK_SHARED_SHORT_TAILS: the members' own ranges are many and short.
  *   prefix_split_tokens  longest piece of a prefix per CTA, 0 = chosen from sm_count.
- *   work_out, combine_out, partial_entries_out  as in gk_attention_plan_build; the low half of a
- *                 record's last word counts the states in front too.
+ *   work_out, combine_out, partial_entries_out  as in gk_attention_plan_build; the states of a prefix
+ *                 stand in front of a block's own and are counted among its splits.
  *   prefix_work_out  [cap*GK_WORK_WORDS] {first listed row, n_rows <= GK_PREFILL_TILES_PER_ITEM *
  *                 (GK_PREFILL_TILE_ROWS / group), part, table_row, kv_begin, kv_end, largest position, 0}
  *   prefix_rows_out  [cap*4] {row, position, entry of query head 0, entries between two parts}; the
@@ -262,12 +263,14 @@ GK_API int gk_prefill_plan_build_two_way(const int32_t* seq, int64_t n_seq, cons
  *
  * gk_shared_prefix_attn_bf16 runs the prefix records on the tensor cores (the kernel of
  * gk_paged_prefill_tc_bf16, its rows gathered) and leaves their states in part_ml / part_o.  DIRECTLY
- * behind it in the same stream gk_paged_attn_extended_multi_bf16 with parts_before[row] = parts of the
- * row's prefix (0 = none) and split_counters attends to the rest and merges: it runs beside the prefix
- * kernel and waits for it only before the merge, so nothing that it reads may be written in between.
+ * behind it in the same stream follows gk_paged_attn_extended_multi_bf16 with the plan's form and
+ * combine records and no split_counters: its attention kernel runs beside the prefix kernel (always a
+ * programmatic dependent launch, whatever gk_set_programmatic_launch says), so nothing that it reads
+ * may be written in between.
  * gk_shared_prefix_check compares table rows: pairs[n_pairs*4] = {row of the group's first member, row
  * of another member, tokens, sequence} (rows through table_rows when not NULL); *verdict receives the
  * smallest sequence that differs (-1: none) and GK_DEV_BAD_METADATA is raised for it. */
+#define GK_SHARED_PREFIX 4        /* the plan has prefix records */
 #define GK_SHARED_ONE_TILE 1
 #define GK_SHARED_SHORT_TAILS 2
 GK_API int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, const int32_t* two_way,
