@@ -44,6 +44,7 @@ struct Totals {
 // Exclusive scans of the batch's new rows and fresh pages into first_row / first_page, and the checks of the whole batch:
 // request ids in range and each named once, lengths that fit the table, rows that fit the outputs, pages that are free.
 // `seen` holds one bit per request.  Called by all threads of a CTA; the arrays are complete when it returns.
+template <int kItems>
 __device__ Totals scan_batch(const ExtendArgs& a, int32_t* first_row, int32_t* first_page, unsigned* seen) {
   __shared__ int64_t warp_rows[32], warp_pages[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -51,20 +52,37 @@ __device__ Totals scan_batch(const ExtendArgs& a, int32_t* first_row, int32_t* f
   __syncthreads();
   Totals t{0, 0, false};
   bool bad = false;
-  for (int base = 0; base < a.batch; base += kThreads) {
-    const int i = base + threadIdx.x;
-    int64_t rows = 0, pages = 0;
-    if (i < a.batch) {
-      const int64_t c = a.lengths[i], n = a.new_tokens[i], r = a.requests[i];
-      if (c < 0 || n < 0 || c > a.context || n > a.context - c || r < 0 || r >= a.n_requests) {
-        bad = true;
-      } else {
-        if (atomicOr(seen + (r >> 5), 1u << (r & 31)) >> (r & 31) & 1) bad = true;      // the same request twice
-        rows = n;
-        pages = (c + n + a.page - 1) / a.page - (c + a.page - 1) / a.page;
-      }
+  // kItems consecutive requests per thread and pass.  Measured: 4096 requests 9.8 us with four, 11.7 us with one; 64 requests
+  // 6.2 and 5.5 us, so the launcher takes one up to 1024 requests.
+  for (int base = 0; base < a.batch; base += kThreads * kItems) {
+    const int first = base + threadIdx.x * kItems;
+    int64_t c[kItems], n[kItems], r[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const bool in = first + k < a.batch;
+      c[k] = in ? a.lengths[first + k] : 0;
+      n[k] = in ? a.new_tokens[first + k] : 0;
+      r[k] = in ? a.requests[first + k] : -1;
     }
-    int64_t r_sum = rows, p_sum = pages;
+    int64_t rows[kItems], pages[kItems], r_sum = 0, p_sum = 0;
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      rows[k] = pages[k] = 0;
+      if (first + k < a.batch) {
+        if (c[k] < 0 || n[k] < 0 || c[k] > a.context || n[k] > a.context - c[k] || r[k] < 0 || r[k] >= a.n_requests) {
+          bad = true;
+        } else {
+          if (atomicOr(seen + (r[k] >> 5), 1u << (r[k] & 31)) >> (r[k] & 31) & 1) bad = true;      // the same request twice
+          rows[k] = n[k];
+          // lengths fit the table and with it 32 bits
+          const unsigned page = (unsigned)a.page;
+          pages[k] = ((unsigned)(c[k] + n[k]) + (page - 1)) / page - ((unsigned)c[k] + (page - 1)) / page;
+        }
+      }
+      r_sum += rows[k];
+      p_sum += pages[k];
+    }
+    const int64_t r_mine = r_sum, p_mine = p_sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t r_up = __shfl_up_sync(0xffffffffu, r_sum, d), p_up = __shfl_up_sync(0xffffffffu, p_sum, d);
@@ -92,11 +110,17 @@ __device__ Totals scan_batch(const ExtendArgs& a, int32_t* first_row, int32_t* f
       warp_pages[lane] = p;
     }
     __syncthreads();
-    if (i < a.batch) {
-      // cut to 32 bits: a batch whose totals do not fit is refused below and nothing reads these
-      first_row[i] = (int32_t)(t.rows + (warp ? warp_rows[warp - 1] : 0) + r_sum - rows);
-      first_page[i] = (int32_t)(t.pages + (warp ? warp_pages[warp - 1] : 0) + p_sum - pages);
-    }
+    // cut to 32 bits: a batch whose totals do not fit is refused below and nothing reads these
+    int64_t row = t.rows + (warp ? warp_rows[warp - 1] : 0) + r_sum - r_mine;
+    int64_t page = t.pages + (warp ? warp_pages[warp - 1] : 0) + p_sum - p_mine;
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+      if (first + k < a.batch) {
+        first_row[first + k] = (int32_t)row;
+        first_page[first + k] = (int32_t)page;
+        row += rows[k];
+        page += pages[k];
+      }
     t.rows += warp_rows[31];
     t.pages += warp_pages[31];
     __syncthreads();
@@ -155,19 +179,20 @@ __device__ void expand_batch(const ExtendArgs& a, const Totals& t, const int32_t
   }
 }
 
+template <int kItems>
 __global__ void __launch_bounds__(kThreads) extend_kernel(const ExtendArgs a) {
   extern __shared__ int32_t shared_words[];
   wait_for_predecessor();
   int32_t* first_row = shared_words;
   int32_t* first_page = first_row + a.batch;
-  const Totals t = scan_batch(a, first_row, first_page, reinterpret_cast<unsigned*>(first_page + a.batch));
+  const Totals t = scan_batch<kItems>(a, first_row, first_page, reinterpret_cast<unsigned*>(first_page + a.batch));
   expand_batch(a, t, first_row, first_page);
 }
 
 __global__ void __launch_bounds__(kThreads) extend_scan_kernel(const ExtendArgs a) {
   extern __shared__ int32_t shared_words[];
   wait_for_predecessor();
-  const Totals t = scan_batch(a, a.workspace, a.workspace + a.batch, reinterpret_cast<unsigned*>(shared_words));
+  const Totals t = scan_batch<4>(a, a.workspace, a.workspace + a.batch, reinterpret_cast<unsigned*>(shared_words));
   if (threadIdx.x == 0) {
     int64_t* verdict = reinterpret_cast<int64_t*>(a.workspace + 2 * (int64_t)a.batch);
     verdict[0] = t.rows;
@@ -214,10 +239,12 @@ extern "C" int gk_extend_requests(int32_t* table, int64_t n_requests, int64_t co
   const unsigned ctas = (unsigned)std::min<int64_t>(148, (std::max(rows, batch) + kThreads - 1) / kThreads);
   if (batch <= kOneLaunchBatch) {
     const size_t bytes = (size_t)batch * 8 + seen_bytes;
-    static std::atomic<bool> configured[64];
-    const int ready = opt_in_shared_memory(extend_kernel, kOneLaunchBatch * 8 + (int)(kMaxRequests / 8), configured);
+    const bool single = batch <= kThreads;
+    static std::atomic<bool> configured[2][64];
+    const int ready = opt_in_shared_memory(single ? extend_kernel<1> : extend_kernel<4>,
+                                           kOneLaunchBatch * 8 + (int)(kMaxRequests / 8), configured[single]);
     if (ready != GK_OK) return ready;
-    launch_after_predecessor(extend_kernel, dim3(ctas), dim3(kThreads), bytes, s, a);
+    launch_after_predecessor(single ? extend_kernel<1> : extend_kernel<4>, dim3(ctas), dim3(kThreads), bytes, s, a);
     return check_launch();
   }
   launch_after_predecessor(extend_scan_kernel, dim3(1), dim3(kThreads), seen_bytes, s, a);

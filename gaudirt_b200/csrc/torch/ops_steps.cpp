@@ -108,17 +108,24 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
                   batch <= 65536 && mapping.size(0) <= 262144,
               "GaudiRT paged allocator: unsupported page size, row count or request count");
   c10::cuda::CUDAGuard guard(device);
-  // straight from the caching allocator: six outputs through the dispatcher cost the host as much as the launch
+  // One block for the six outputs: through the dispatcher one by one they cost the host as much as the launch.
+  const auto block = at::Tensor(at::detail::empty_cuda({(batch + 1) * 8 + (3 * rows + batch + 1) * 4}, at::kByte, device, c10::nullopt));
+  int64_t cursor = 0;
   auto vector = [&](int64_t n, at::ScalarType type) {
-    return at::Tensor(at::detail::empty_cuda({n}, type, device, c10::nullopt));
+    const auto meta = at::scalarTypeToTypeMeta(type);
+    auto out = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), meta);
+    out.unsafeGetTensorImpl()->set_storage_offset(cursor / static_cast<int64_t>(meta.itemsize()));
+    out.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    cursor += n * static_cast<int64_t>(meta.itemsize());
+    return out;
   };
+  auto next_lengths = vector(batch, at::kLong), next_used = vector(1, at::kLong);
   auto locations = vector(rows, at::kInt), positions = vector(rows, at::kInt), row_requests = vector(rows, at::kInt);
   auto row_offsets = vector(batch + 1, at::kInt);
-  auto next_lengths = vector(batch, at::kLong), next_used = vector(1, at::kLong);
   uint64_t bytes = 0;
   check_status(gk_extend_requests_workspace_bytes(batch, &bytes), "paged allocator");
   at::Tensor workspace;
-  if (bytes > 0) workspace = vector(static_cast<int64_t>(bytes), at::kByte);
+  if (bytes > 0) workspace = at::Tensor(at::detail::empty_cuda({static_cast<int64_t>(bytes)}, at::kByte, device, c10::nullopt));
   check_status(gk_extend_requests(mapping.data_ptr<int32_t>(), mapping.size(0), mapping.size(1), mapping.stride(0),
                                   batch_requests.data_ptr<int32_t>(), lengths.data_ptr<int64_t>(),
                                   new_tokens.data_ptr<int32_t>(), batch, free_pages.data_ptr<int64_t>(), free_pages.numel(),
