@@ -332,17 +332,24 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const
 
     // ---- scale, softcap, mask -----------------------------------------------------------
     const int tok0 = kv_begin + (warp + i * WARPS) * kGroupTokens;
-    if (capped) {
-      const float inv = p.scale / p.softcap;
+    if (EXT && capped) {
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[nt][e] = p.softcap * tanhf(sc[nt][e] * inv);
+        for (int e = 0; e < 4; ++e) sc[nt][e] = capped_score(sc[nt][e], 2.f * kLog2e * p.scale / p.softcap, p.softcap * kLog2e);
+    } else {
+      if (capped) {
+        const float inv = p.scale / p.softcap;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nt][e] = p.softcap * tanhf(sc[nt][e] * inv);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[nt][e] *= to_log2;
     }
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sc[nt][e] *= to_log2;
     if (EXT && p.slopes) {
       // -slope * |position - key|: the distance is taken in integers and rounded once (exact below 2^24)
       const float d0 = (float)(tok0 + 2 * t - pos0), d1 = (float)(tok0 + 2 * t - pos1);

@@ -135,16 +135,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// softcap * tanh(scale * s / softcap) in log2 units, from tanh(x) = 1 - 2 / (exp(2x) + 1): `e` is 2 log2(e) scale / softcap
-// and `c` softcap * log2(e).  Both ends come out exactly (exp2 gives 0 or infinity).  The absolute error is a few 2^-22 of
-// the cap (three fp32 operations on values of at most 2), next to which a probability's rounding to bf16 is 2^-9; a score
-// enters an exponential, so its absolute error is what counts, not the relative one near zero.
-__device__ __forceinline__ float capped_score(float s, float e, float c) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(fast_exp2(s * e) + 1.f));
-  return fmaf(-2.f * c, r, c);
-}
-
 // BIASED: a distance bias and row limits.
 // FORM: kRowsForm is the kernel described above.  The shared forms attend to keys that several sequences have in common:
 // the rows of a record are listed, every listed row sees all of the record's keys but for its window, and the state
@@ -154,8 +144,10 @@ __device__ __forceinline__ float capped_score(float s, float e, float c) {
 // the tensor pipe still has two independent chains although a K/V tile is read for one query tile only, Q.K^T runs two KV
 // tiles ahead, and the room of the second query tile is a third K stage; the two chains' states are merged through shared
 // memory at the end.
+// CAP: the scores are capped (the biased and the shared kernels are built with and without: the common path of one that has
+// the cap's code beside it ran 5 % slower).  The plain kernel decides at run time.
 constexpr int kRowsForm = 0, kWideForm = 1, kNarrowForm = 2;
-template <int D, bool BIASED, int FORM>
+template <int D, bool BIASED, int FORM, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const PrefillParams p,
                                                                        const __grid_constant__ CUtensorMap map_k,
                                                                        const __grid_constant__ CUtensorMap map_v) {
@@ -321,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     const float slope = BIASED && p.slopes && pr < mv ? __ldg(p.slopes + head * G + pr % G) * kLog2e : 0.f;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + 256 + t * D + lane_base;
-    const bool capped = p.softcap > 0.f;
+    const bool capped = BIASED || SHARED ? CAP : p.softcap > 0.f;
     const float to_log2 = capped ? kLog2e : p.scale * kLog2e;
     const float cap_in = capped ? p.scale / p.softcap : 0.f;
     const float cap_exp = 2.f * kLog2e * cap_in, cap_log2 = p.softcap * kLog2e;     // see capped_score
@@ -349,10 +341,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       // the two passes below stay one short piece of code (the instruction cache is what this kernel
       // runs out of first when every variant is unrolled 128 times).
       float mult = to_log2;
-      // Slopes too steep for the estimate of the maximum below go the exact way of the uncommon tiles.
-      const bool rewrite = capped || ragged || (BIASED && steep);
+      // Tiles whose scores cannot stay what they are go through an exact rewrite: a cap, slopes too steep for the estimate
+      // of the maximum below, and biased rows that see keys behind them (there the bias falls again).
+      const bool rewrite = BIASED || SHARED ? capped || (BIASED && p.slopes && (steep || (p.row_limits && tile_end > tile_first_pos + 1)))
+                                            : capped || ragged;
       const float fast_slope = BIASED && !rewrite ? slope : 0.f;
-      if (rewrite) {
+      if (rewrite || ragged) {
         if (BIASED || SHARED) {
           // The keys a row sees are one interval: a key is in it when its distance from the first one is at most `span`.
           int low = p.window > 0 ? pos - p.window + 1 : 0, span = min(lim, kv_end - 1) - low;
@@ -361,18 +355,47 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
             span = 0;
           }
           const int rel = tok0 - low;
+          if (rewrite) {
 #pragma unroll 1
-          for (int c = 0; c < kScoreChunks; ++c) {
-            uint32_t r[32];
-            tmem_ld32(s_addr + c * 32, r);
+            for (int c = 0; c < kScoreChunks; ++c) {
+              uint32_t r[32];
+              tmem_ld32(s_addr + c * 32, r);
+              float big = 0.f;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              float v = __uint_as_float(r[e]);
-              v = capped ? capped_score(v, cap_exp, cap_log2) : v * to_log2;
-              if (BIASED) v = fmaf(-slope, fabsf(from + (float)(c * 32 + e)), v);
-              r[e] = __float_as_uint((unsigned)(rel + c * 32 + e) <= (unsigned)span ? v : -CUDART_INF_F);
+              for (int e = 0; e < 32; e += 2) big = max3(big, fabsf(__uint_as_float(r[e])), fabsf(__uint_as_float(r[e + 1])));
+              if (capped && __all_sync(0xffffffffu, big * cap_in <= 0.5f)) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                  float2 v = capped_small_scores(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), cap_in, p.scale * kLog2e);
+                  if (BIASED) {
+                    v.x = fmaf(-slope, fabsf(from + (float)(c * 32 + e)), v.x);
+                    v.y = fmaf(-slope, fabsf(from + (float)(c * 32 + e + 1)), v.y);
+                  }
+                  r[e] = __float_as_uint((unsigned)(rel + c * 32 + e) <= (unsigned)span ? v.x : -CUDART_INF_F);
+                  r[e + 1] = __float_as_uint((unsigned)(rel + c * 32 + e + 1) <= (unsigned)span ? v.y : -CUDART_INF_F);
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  float v = __uint_as_float(r[e]);
+                  v = capped ? capped_score(v, cap_exp, cap_log2) : v * to_log2;
+                  if (BIASED) v = fmaf(-slope, fabsf(from + (float)(c * 32 + e)), v);
+                  r[e] = __float_as_uint((unsigned)(rel + c * 32 + e) <= (unsigned)span ? v : -CUDART_INF_F);
+                }
+              }
+              tmem_st32(s_addr + c * 32, r);
             }
-            tmem_st32(s_addr + c * 32, r);
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < kScoreChunks; ++c) {
+              const int at = rel + c * 32;
+              if (!__any_sync(0xffffffffu, at < 0 || at + 31 > span)) continue;      // every row of the warp sees all 32
+              uint32_t r[32];
+              tmem_ld32(s_addr + c * 32, r);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) r[e] = (unsigned)(at + e) <= (unsigned)span ? r[e] : 0xff800000u;      // -infinity
+              tmem_st32(s_addr + c * 32, r);
+            }
           }
         } else {
 #pragma unroll 1
@@ -384,7 +407,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
             float v = __uint_as_float(r[e]);
             if (capped) v = p.softcap * tanhf(v * cap_in);
             v *= to_log2;
-            if (BIASED) v = fmaf(-slope, fabsf(from + (float)(c * 32 + e)), v);
             const int tok = tok0 + c * 32 + e;
             const bool seen = tok < kv_end && tok <= lim && (p.window <= 0 || tok > pos - p.window);
             r[e] = __float_as_uint(seen ? v : -CUDART_INF_F);
@@ -392,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
           tmem_st32(s_addr + c * 32, r);
         }
         }
-        mult = 1.f;
+        if (rewrite) mult = 1.f;
       }
       // ---- the whole row comes in once (up to 128 registers) and stays until it has become P ----
       uint32_t sr[kScoreChunks][32];
@@ -794,10 +816,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
 }
 
-template <int D, bool BIASED, int FORM>
+template <int D, bool BIASED, int FORM, bool CAP>
 int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream_t stream) {
   static std::atomic<bool> configured[64];
-  const int ready = opt_in_shared_memory(paged_prefill_tc_kernel<D, BIASED, FORM>, Geo<D>::kSmemBytes, configured);
+  const int ready = opt_in_shared_memory(paged_prefill_tc_kernel<D, BIASED, FORM, CAP>, Geo<D>::kSmemBytes, configured);
   if (ready != GK_OK) return ready;
   {
     // Never launch if the register pool of this build cannot satisfy the budgets (the kernel would hang).
@@ -805,7 +827,7 @@ int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream
     int regs = launch_regs.load(std::memory_order_acquire);
     if (regs < 0) {
       cudaFuncAttributes attr;
-      if (cudaFuncGetAttributes(&attr, paged_prefill_tc_kernel<D, BIASED, FORM>) != cudaSuccess) return check_launch();
+      if (cudaFuncGetAttributes(&attr, paged_prefill_tc_kernel<D, BIASED, FORM, CAP>) != cudaSuccess) return check_launch();
       regs = attr.numRegs;
       launch_regs.store(regs, std::memory_order_release);
     }
@@ -825,9 +847,9 @@ int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream
   const int64_t ctas = n_work * p.kv_heads * (Geo<D>::kTiles == 2 ? 1 : 2);
   if (ctas > 0x7fffffffLL) return GK_ERR_UNSUPPORTED;
   if (FORM == kRowsForm)
-    paged_prefill_tc_kernel<D, BIASED, FORM><<<(unsigned)ctas, kThreads, Geo<D>::kSmemBytes, stream>>>(p, map_k, map_v);
+    paged_prefill_tc_kernel<D, BIASED, FORM, CAP><<<(unsigned)ctas, kThreads, Geo<D>::kSmemBytes, stream>>>(p, map_k, map_v);
   else
-    launch_programmatic(true, paged_prefill_tc_kernel<D, BIASED, FORM>, dim3((unsigned)ctas), dim3(kThreads),
+    launch_programmatic(true, paged_prefill_tc_kernel<D, BIASED, FORM, CAP>, dim3((unsigned)ctas), dim3(kThreads),
                         Geo<D>::kSmemBytes, stream, p, map_k, map_v);
   return check_launch();
 }
@@ -844,11 +866,17 @@ struct PrefillExtras {
   float* part_o = nullptr;
 };
 
-template <bool BIASED, int FORM>
+template <bool BIASED, int FORM, bool CAP>
 int launch_prefill_dim(PrefillParams& p, int head_dim, int64_t n_work, int page_tokens, cudaStream_t stream) {
-  if (head_dim == 64) return launch_prefill<64, BIASED, FORM>(p, n_work, page_tokens, stream);
-  if (head_dim == 256) return launch_prefill<256, BIASED, FORM == kNarrowForm ? kWideForm : FORM>(p, n_work, page_tokens, stream);
-  return launch_prefill<128, BIASED, FORM>(p, n_work, page_tokens, stream);
+  if (head_dim == 64) return launch_prefill<64, BIASED, FORM, CAP>(p, n_work, page_tokens, stream);
+  if (head_dim == 256) return launch_prefill<256, BIASED, FORM == kNarrowForm ? kWideForm : FORM, CAP>(p, n_work, page_tokens, stream);
+  return launch_prefill<128, BIASED, FORM, CAP>(p, n_work, page_tokens, stream);
+}
+
+template <bool BIASED, int FORM>
+int launch_prefill_cap(PrefillParams& p, int head_dim, int64_t n_work, int page_tokens, cudaStream_t stream) {
+  return p.softcap > 0.f ? launch_prefill_dim<BIASED, FORM, true>(p, head_dim, n_work, page_tokens, stream)
+                         : launch_prefill_dim<BIASED, FORM, false>(p, head_dim, n_work, page_tokens, stream);
 }
 
 int prefill_entry(const void* q, int64_t q_row_stride, const void* pool_k, const void* pool_v, int64_t slots,
@@ -904,13 +932,13 @@ int prefill_entry(const void* q, int64_t q_row_stride, const void* pool_k, const
   p.part_o = extras.part_o;
   cudaStream_t at = reinterpret_cast<cudaStream_t>(stream);
   if (shared && extras.narrow)
-    return p.slopes ? launch_prefill_dim<true, kNarrowForm>(p, head_dim, n_work, page_tokens, at)
-                    : launch_prefill_dim<false, kNarrowForm>(p, head_dim, n_work, page_tokens, at);
+    return p.slopes ? launch_prefill_cap<true, kNarrowForm>(p, head_dim, n_work, page_tokens, at)
+                    : launch_prefill_cap<false, kNarrowForm>(p, head_dim, n_work, page_tokens, at);
   if (shared)
-    return p.slopes ? launch_prefill_dim<true, kWideForm>(p, head_dim, n_work, page_tokens, at)
-                    : launch_prefill_dim<false, kWideForm>(p, head_dim, n_work, page_tokens, at);
-  return p.slopes || p.row_limits ? launch_prefill_dim<true, kRowsForm>(p, head_dim, n_work, page_tokens, at)
-                                  : launch_prefill_dim<false, kRowsForm>(p, head_dim, n_work, page_tokens, at);
+    return p.slopes ? launch_prefill_cap<true, kWideForm>(p, head_dim, n_work, page_tokens, at)
+                    : launch_prefill_cap<false, kWideForm>(p, head_dim, n_work, page_tokens, at);
+  return p.slopes || p.row_limits ? launch_prefill_cap<true, kRowsForm>(p, head_dim, n_work, page_tokens, at)
+                                  : launch_prefill_dim<false, kRowsForm, false>(p, head_dim, n_work, page_tokens, at);
 }
 
 }  // namespace
