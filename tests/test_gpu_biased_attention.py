@@ -162,3 +162,45 @@ def test_refusals(rt):
         fresh()._set_prefix_mask_([0])
     assert torch.equal(pool, before)
     assert rt._C._take_device_status() == 0
+
+
+def test_same_bits_on_every_launch(rt):
+    step = steps.plain_step([500, 20, 0, 260], [1, 330, 140, 2], 8, 2, 128, 16, seed=41, two_way=[0, 200, 140, 0])
+    slopes = steps.slopes_of(8).to(DEV)
+    md = metadata(rt, step)
+    _, kp, vp = pools(step, stored=True)
+    call = lambda: torch.ops.gaudirt._paged_attn_biased(step.q.to(DEV), None, None, kp, vp, md, slopes, 128, step.scale)  # noqa: E731
+    first = call()
+    assert all(torch.equal(call(), first) for _ in range(20))
+
+
+def test_rising_bias(rt):
+    """Negative slopes: the farthest keys weigh most."""
+    step = steps.plain_step([300, 3], [1, 200], 8, 2, 128, 16, seed=43)
+    slopes = -steps.slopes_of(8) / 16
+    _, kp, vp = pools(step, stored=True)
+    out = torch.ops.gaudirt._paged_attn_biased(step.q.to(DEV), None, None, kp, vp, metadata(rt, step), slopes.to(DEV), 128,
+                                               step.scale)
+    steps.check(out, *steps.attend64(step, step.stored_pool(), slopes=slopes))
+
+
+def test_captured_and_replayed(rt):
+    step = steps.plain_step([70, 0, 12], [1, 90, 2], 8, 2, 64, 16, seed=8, two_way=[0, 50, 0])
+    slopes = steps.slopes_of(8).to(DEV)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        md = metadata(rt, step)
+        _, kp, vp = pools(step)
+        q, k, v = step.q.to(DEV), step.k.to(DEV), step.v.to(DEV)
+        eager = torch.ops.gaudirt._paged_attn_biased(q, k, v, kp, vp, md, slopes, 64, step.scale)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = torch.ops.gaudirt._paged_attn_biased(q, k, v, kp, vp, md, slopes, 64, step.scale)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, eager)
+        stream.synchronize()
+    with pytest.raises(RuntimeError, match="stream"):          # a plan belongs to the stream it was built on
+        torch.ops.gaudirt._paged_attn_biased(q, k, v, kp, vp, md, slopes, 64, step.scale)

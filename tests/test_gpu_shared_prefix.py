@@ -216,3 +216,74 @@ def test_prefix_of_no_tokens_and_empty_groups(rt):
     _, kp, vp = pools(step, stored=True)
     out = torch.ops.gaudirt._paged_attn_stored(step.q.to(DEV), kp, vp, md, 128, step.scale)
     steps.check(out, *steps.attend64(step, step.stored_pool()))
+
+
+@pytest.mark.parametrize("geometry", [(8, 2, 128), (6, 2, 64), (8, 1, 256)])
+def test_layers_in_a_row_give_the_same_bits(rt, geometry):
+    """Prefix, tail and combine of one layer run beside each other and share one split state with the next layer's: many
+    layers without a wait in between, the KV store riding in the tail launch, a prefill chunk in the step."""
+    step = steps.shared_step([1500, 700], [(0, 30, 1), (1, 400, 1), (0, 0, 1), (-1, 900, 1), (1, 9, 1), (0, 250, 2), (1, 3, 90)],
+                             *geometry, 16, seed=17)
+    md = shared_metadata(rt, step)
+    q, k, v = step.q.to(DEV), step.k.to(DEV), step.v.to(DEV)
+    layers = [pools(step) for _ in range(3)]
+    for i, (pool, _, _) in enumerate(layers):
+        pool.mul_(1.0 - 0.25 * i)
+    first = [None] * 3
+    for turn in range(60):
+        _, kp, vp = layers[turn % 3]
+        out = torch.ops.gaudirt.paged_attn(q, k, v, kp, vp, md, step.head_dim, step.scale)
+        if first[turn % 3] is None:
+            first[turn % 3] = out
+        else:
+            assert torch.equal(out, first[turn % 3]), turn
+    steps.check(first[0], *steps.attend64(step, step.stored_pool()))
+    assert rt._C._take_device_status() == 0
+
+
+def test_everything_at_once(rt):
+    """Shared prefixes, a two-way prefix, a distance bias, a cap and a window in one mixed step."""
+    step = steps.shared_step([320], [(0, 40, 1), (0, 0, 3), (-1, 90, 1), (0, 100, 1), (0, 7, 80)], 12, 4, 128, 16, seed=23)
+    step.two_way = [0, 323, 0, 421, 400]
+    md = shared_metadata(rt, step)
+    md._set_prefix_mask_(step.two_way)
+    slopes = steps.slopes_of(12)
+    _, kp, vp = pools(step)
+    out = torch.ops.gaudirt._paged_attn_biased(step.q.to(DEV), step.k.to(DEV), step.v.to(DEV), kp, vp, md, slopes.to(DEV), 128,
+                                               step.scale, 8.0, 300)
+    assert md._last_plan_prefix_records() > 0
+    steps.check(out, *steps.attend64(step, step.stored_pool(), 8.0, 300, slopes))
+
+
+@pytest.mark.parametrize("softcap", [0.05, 0.5, 2.0, 1000.0])
+def test_caps_from_tight_to_loose(rt, softcap):
+    """Scores far inside, around and far outside the cap: both ways of computing it."""
+    step = steps.shared_step([300], [(0, 40, 1), (0, 0, 1), (-1, 90, 1)], 8, 2, 128, 16, seed=29)
+    md = shared_metadata(rt, step)
+    _, kp, vp = pools(step, stored=True)
+    out = torch.ops.gaudirt._paged_attn_stored(step.q.to(DEV), kp, vp, md, 128, step.scale, softcap)
+    steps.check(out, *steps.attend64(step, step.stored_pool(), softcap))
+
+
+def test_many_short_tails(rt):
+    """Enough rows for the form with two warps per tail, of one and of several splits."""
+    step = steps.shared_step([256], [(0, (i * 37) % 200, 1) for i in range(130)], 32, 8, 128, 32, seed=31)
+    for splits in (0, 64):
+        md = shared_metadata(rt, step, splits=splits)
+        _, kp, vp = pools(step, stored=True)
+        out = torch.ops.gaudirt._paged_attn_stored(step.q.to(DEV), kp, vp, md, 128, step.scale)
+        steps.check(out, *steps.attend64(step, step.stored_pool()))
+
+
+def test_scheduler_owned_metadata(rt):
+    """A table the scheduler vouches for: nothing is compared, the store is a launch of its own."""
+    step = steps.shared_step([96], [(0, 21, 1), (0, 0, 1), (0, 64, 2)], 8, 2, 128, 16, seed=6)
+    batch = torch.arange(3, dtype=torch.int32, device=DEV)
+    md = rt.PagedMetadata._from_scheduler(step.locations.to(DEV), batch, step.positions.to(torch.int32).to(DEV),
+                                          step.mapping.to(DEV), step.cached, step.lengths, step.slots, None, 0)
+    md._share_prefixes_(step.groups, step.prefixes)
+    md._set_prefix_sharing(1, 0)
+    pool, kp, vp = pools(step)
+    out = torch.ops.gaudirt.paged_attn(step.q.to(DEV), step.k.to(DEV), step.v.to(DEV), kp, vp, md, 128, step.scale)
+    assert torch.equal(pool.cpu().view(torch.int16), step.stored_pool().view(torch.int16))
+    steps.check(out, *steps.attend64(step, step.stored_pool()))

@@ -192,3 +192,17 @@ def test_launch_arguments_are_judged_on_the_host():
         args = list(attend)
         args[at] = value
         assert lib.gk_shared_prefix_attn_bf16(*args) == UNSUPPORTED, at
+    extended = [one, 1024, None, None, 0, 0, None, one, one, 64, one, 16, 1, 1, None, one, 1, one, 1, (C.c_void_p * 1)(4096), 1, 1024,
+                one, one, None, None, None, 4, 1.0, 0.0, -1, 8, 2, 128, None, None]
+    for at, value in ((0, None), (15, None), (17, None), (18, -1), (16, 0), (22, None), (24, one), (25, C.c_void_p(4097)),
+                      (26, C.c_void_p(4098)), (27, 8), (28, 0.0), (2, one)):
+        args = list(extended)
+        args[at] = value
+        assert lib.gk_paged_attn_extended_multi_bf16(*args) == INVALID, at
+    for at, value in ((31, 34), (33, 96)):
+        args = list(extended)
+        args[at] = value
+        assert lib.gk_paged_attn_extended_multi_bf16(*args) == UNSUPPORTED, at
+    args = list(extended)
+    args[16] = args[18] = 0                                        # nothing to do is not an error
+    assert lib.gk_paged_attn_extended_multi_bf16(*args) == 0
