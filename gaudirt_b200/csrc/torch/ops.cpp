@@ -7,6 +7,8 @@
 // message raised before any pool write; there is no fallback path.
 #include "ops_common.h"
 
+#include <ATen/cuda/EmptyTensor.h>
+
 namespace gaudirt_b200 {
 
 // ---------------------------------------------------------------------------------------------
@@ -81,7 +83,8 @@ at::Tensor paged_attn_impl(const at::Tensor& query, const c10::optional<at::Tens
   std::vector<void*> outs;
   int64_t out_stride = query.size(1);
   if (pushed.empty()) {
-    output = at::empty({plan.rows, query.size(1)}, query.options().memory_format(at::MemoryFormat::Contiguous));
+    // straight from the caching allocator: the dispatcher's way to the same block costs the host another microsecond
+    output = at::Tensor(at::detail::empty_cuda({plan.rows, query.size(1)}, at::kBFloat16, device, c10::nullopt));
     outs.push_back(output.data_ptr());
   } else {
     TORCH_CHECK(pushed.size() <= GK_MAX_OUTPUTS, "GaudiRT attention: too many gather destinations");

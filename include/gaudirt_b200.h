@@ -151,7 +151,7 @@ GK_API int gk_paged_attn_bf16(const void* q, int64_t q_row_stride, const void* p
                        float* part_o, float scale, float softcap, int window, int q_heads,
                        int kv_heads, int head_dim, int32_t* status, gk_stream_t stream);
 
-/* Programmatic dependent launch (on by default): the attention, combine, norm, rotary and barrier kernels
+/* Programmatic dependent launch (off by default): the attention, combine, norm, rotary and barrier kernels
  * are launched so that the GPU may set them up while the kernel before them in the stream is still
  * running; their first statement waits until that kernel has completed and its writes are visible, so
  * every access keeps plain stream order and only launch latency overlaps.  0 switches back to ordinary
