@@ -436,17 +436,18 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
   // The form of the records (one or two query tiles) and how long a piece of the prefix one CTA takes: the cheapest by a
   // model of the two kernels side by side, in us.  A prefix CTA has an SM to itself for a fixed 7 us and 1.2 us per 128 keys
   // and one query tile, 2.4 us per two (1.0 and 1.9 at head_dim 64, 1.1 per 64 keys at 256).  The members' own CTAs take
-  // 3.5 us and 36 GB/s each; two per SM run on the SMs that the prefix leaves and on all of them once it is done.  Neither
-  // is faster than memory gives the bytes of both.  Every part of a row costs its merge 0.15 us.  So the longer of the two
+  // 3.5 us and 36 GB/s each, two per SM on the SMs that the prefix leaves and on all of them once it is done, never faster
+  // than memory gives their bytes and never more than 50 of them in a us (2048 of 64 KB took 40 us on 84 and on 148 SMs).  Every part of a row costs its merge 0.15 us.  So the longer of the two
   // gets the SMs: measured with 256 members of 4096 + 1024 tokens, 32 CTAs of two tiles or 64 of one 108 us, 128 of one
   // 123 us; with 32 members of 2048 + 256, 32 CTAs 16.7 us, 64 of them 18.4 us, 128 of them 23.7 us.
   bool one_tile = head_dim != 256;
   int64_t piece = prefix_split_tokens;
   if (!shared.empty()) {
-    constexpr double kFixed = 7.0, kTailFixed = 3.5, kTailBytes = 36e3, kMemoryBytes = 5.9e6, kMergePart = 0.15;
+    constexpr double kFixed = 7.0, kTailFixed = 3.5, kTailBytes = 36e3, kMemoryBytes = 5.9e6, kTailsPerUs = 50.0,
+                     kMergePart = 0.15;
     const double one_time = head_dim == 64 ? 1.0 : head_dim == 128 ? 1.2 : 1.1, two_time = head_dim == 64 ? 1.9 : 2.4;
     const double head_bytes = head_dim * 4.0;
-    double all_bytes = 0.0, tail_time = 0.0, tail_longest = 0.0;
+    double all_bytes = 0.0, tail_bytes = 0.0, tail_longest = 0.0;
     int64_t tail_ctas = 0;
     std::vector<int32_t> starts(static_cast<size_t>(n_seq), 0);
     int32_t longest = 0;
@@ -458,14 +459,16 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
     for (int64_t s = 0; s < n_seq; ++s) {
       const int32_t* r = seq + s * 4;
       const int64_t from = std::max<int64_t>(starts[s], window > 0 ? std::max(0, r[2] - window + 1) : 0);
-      const double bytes = (double)((int64_t)r[2] + r[1] - from) * head_bytes, time = kTailFixed + bytes / kTailBytes;
+      const double bytes = (double)((int64_t)r[2] + r[1] - from) * head_bytes;
       const int64_t ctas = (r[1] + GK_MAX_PACKED_ROWS / group_heads - 1) / (GK_MAX_PACKED_ROWS / group_heads) * kv_heads;
-      all_bytes += ctas * bytes;
+      tail_bytes += ctas * bytes;
       tail_ctas += ctas;
-      tail_time += ctas * time;
-      tail_longest = std::max(tail_longest, time);
+      tail_longest = std::max(tail_longest, bytes);
     }
-    const double tail_mean = tail_time / (double)tail_ctas;
+    all_bytes += tail_bytes;
+    const double mean_bytes = tail_bytes / (double)tail_ctas;
+    const double tail_mean = kTailFixed + mean_bytes / kTailBytes;
+    tail_longest = kTailFixed + tail_longest / kTailBytes;
     auto estimate = [&](bool one, int64_t tiles) {
       int64_t ctas = 0, most_parts = 0;
       double busy = 0.0, slowest = 0.0;
@@ -484,8 +487,11 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
       const double slots = 2.0 * (double)std::max<int64_t>(0, sm_count - ctas);
       double tails = tail_longest;
       if ((double)tail_ctas > slots) {
-        const double left = std::max(0.0, (double)tail_ctas - std::floor(prefix / tail_mean) * slots);
-        tails = left > 0.0 ? prefix + std::max(1.0, left / (2.0 * sm_count)) * tail_mean : prefix;
+        const double beside = std::min(std::floor(prefix / tail_mean) * slots, prefix * kTailsPerUs);
+        const double left = std::max(0.0, (double)tail_ctas - beside);
+        tails = prefix;
+        if (left > 0.0)
+          tails += std::max({std::max(1.0, left / (2.0 * sm_count)) * tail_mean, left * mean_bytes / kMemoryBytes, left / kTailsPerUs});
       }
       return std::max({prefix, tails, all_bytes / kMemoryBytes}) + kMergePart * (double)most_parts;
     };
