@@ -227,8 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh->tmem_base)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
   }
-  // The shared forms may be set up while the kernel before them runs.  The attention kernel behind them is released only
-  // once that kernel has completed: it reads the queries and the pool without waiting for this one.
+  // The attention kernel behind the shared forms is released once the kernel before them has completed: it reads the queries
+  // and the pool without waiting for this one.
   if (SHARED) asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;\n" ::: "memory");
   tc_fence_before();
   __syncthreads();                                       // barriers and the TMEM allocation are in place
@@ -849,8 +849,8 @@ int launch_prefill(PrefillParams& p, int64_t n_work, int page_tokens, cudaStream
   if (FORM == kRowsForm)
     paged_prefill_tc_kernel<D, BIASED, FORM, CAP><<<(unsigned)ctas, kThreads, Geo<D>::kSmemBytes, stream>>>(p, map_k, map_v);
   else
-    launch_programmatic(true, paged_prefill_tc_kernel<D, BIASED, FORM, CAP>, dim3((unsigned)ctas), dim3(kThreads),
-                        Geo<D>::kSmemBytes, stream, p, map_k, map_v);
+    launch_after_predecessor(paged_prefill_tc_kernel<D, BIASED, FORM, CAP>, dim3((unsigned)ctas), dim3(kThreads),
+                             Geo<D>::kSmemBytes, stream, p, map_k, map_v);
   return check_launch();
 }
 

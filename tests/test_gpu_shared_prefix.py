@@ -287,3 +287,20 @@ def test_scheduler_owned_metadata(rt):
     out = torch.ops.gaudirt.paged_attn(step.q.to(DEV), step.k.to(DEV), step.v.to(DEV), kp, vp, md, 128, step.scale)
     assert torch.equal(pool.cpu().view(torch.int16), step.stored_pool().view(torch.int16))
     steps.check(out, *steps.attend64(step, step.stored_pool()))
+
+
+def test_programmatic_launch_changes_no_bits(rt):
+    """The prefix kernel set up while the kernel before it still runs, over several layers."""
+    step = steps.shared_step([600], [(0, 30, 1), (0, 0, 1), (-1, 300, 1), (0, 250, 2)], 8, 2, 128, 16, seed=37)
+    md = shared_metadata(rt, step)
+    pool, kp, vp = pools(step)
+    q, k, v = step.q.to(DEV), step.k.to(DEV), step.v.to(DEV)
+    call = lambda: torch.ops.gaudirt.paged_attn(q, k, v, kp, vp, md, 128, step.scale)  # noqa: E731
+    first = call()
+    try:
+        assert rt.abi.lib().gk_set_programmatic_launch(1) == 0
+        outs = [call() for _ in range(20)]
+    finally:
+        rt.abi.lib().gk_set_programmatic_launch(0)
+    assert all(torch.equal(out, first) for out in outs)
+    steps.check(first, *steps.attend64(step, step.stored_pool()))
