@@ -391,7 +391,8 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
                                            int64_t work_cap, int64_t* n_work_out, int32_t* combine_out,
                                            int64_t combine_cap, int64_t* n_combine_out, int64_t* partial_entries_out,
                                            int32_t* prefix_work_out, int64_t prefix_work_cap, int64_t* n_prefix_work_out,
-                                           int32_t* prefix_rows_out, int64_t prefix_rows_cap, int64_t* n_prefix_rows_out) {
+                                           int32_t* prefix_rows_out, int64_t prefix_rows_cap,
+                                           int64_t* n_prefix_rows_out) try {
   if (!seq || n_seq <= 0 || n_groups < 0 || (n_groups > 0 && (!groups || !prefix_tokens)) || prefix_split_tokens < 0 ||
       min_saved_bytes < 0 || !form_out || !n_prefix_work_out || !n_prefix_rows_out || sm_count <= 0 || (window != -1 && window <= 0))
     return GK_ERR_INVALID_ARGUMENT;
@@ -572,6 +573,8 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
     std::copy(rows[i].begin(), rows[i].end(), prefix_rows_out + i * 4);
   }
   return GK_OK;
+} catch (...) {
+  return GK_ERR_CAPACITY;     // the lists of a plan did not fit into memory; nothing leaves a C entry by exception
 }
 
 namespace {
@@ -634,7 +637,9 @@ extern "C" int gk_prefill_plan_build(const int32_t* seq, int64_t n_seq, int q_he
 
 extern "C" int gk_prefill_plan_build_two_way(const int32_t* seq, int64_t n_seq, const int32_t* two_way, int q_heads,
                                              int kv_heads, int window, int min_rows, int32_t* work_out, int64_t work_cap,
-                                             int64_t* n_work_out, int32_t* rest_seq_out, int64_t* n_rest_out) {
+                                             int64_t* n_work_out, int32_t* rest_seq_out, int64_t* n_rest_out) try {
   return prefill_plan_build(seq, n_seq, two_way, q_heads, kv_heads, window, min_rows, work_out, work_cap, n_work_out,
                             rest_seq_out, n_rest_out);
+} catch (...) {
+  return GK_ERR_CAPACITY;
 }

@@ -144,6 +144,11 @@ def test_refusals():
     assert build(seq, [0, 0], [90], 34, 2, 128) == UNSUPPORTED
     assert build(seq, [0, 0], [90], 8, 2, 128, shrink=1) == CAPACITY
     assert build([(0, 1, 2**31 - 1, 0), (1, 1, 5, 1)], [0, 0], [5], 8, 2, 128) == INVALID
+    # lists that cannot be held end as an error code, not as an exception through a C entry
+    lib, sizes = abi.lib(), [C.byref(C.c_int64()) for _ in range(5)]
+    one = np.array(seq, dtype=np.int32)
+    assert lib.gk_shared_prefix_plan_build(ptr(one), 2, None, ptr(one), ptr(one), 2**60, 8, 2, 128, -1, 148, 0, 0, 0, C.byref(C.c_int()),
+                                           None, 0, sizes[0], None, 0, sizes[1], sizes[2], None, 0, sizes[3], None, 0, sizes[4]) == CAPACITY
 
 
 def test_two_way_prefill_records():
