@@ -124,18 +124,20 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }
 
 // softcap * tanh(scale * s / softcap) in log2 units, from tanh(x) = 1 - 2 / (exp(2x) + 1): `e` is 2 log2(e) scale / softcap
-// and `c` softcap * log2(e).  Both ends come out exactly (exp2 gives 0 or infinity).  The absolute error is a few 2^-22 of
-// the cap (three fp32 operations on values of at most 2), next to which a probability's rounding to bf16 is 2^-9; a score
-// enters an exponential, so its absolute error is what counts, not the relative one near zero.
-__device__ __forceinline__ float capped_score(float s, float e, float c) {
+// and `c` softcap * log2(e).  Both ends come out exactly (exp2 gives 0 or infinity).  The absolute error is a few 2^-23 of
+// the cap whatever the score: a few 2^-22 of the result where |scale * s / softcap| is above 1/2, and 2^-14 (of a score
+// that enters an exponential, where a probability's rounding to bf16 is 2^-9) up to kTightCap.  At a cap of 10^6 it would be
+// 0.2 of a score of ordinary size.
+constexpr float kTightCap = 256.f;
+__device__ __forceinline__ float capped_large_score(float s, float e, float c) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(fast_exp2(s * e) + 1.f));
   return fmaf(-2.f * c, r, c);
 }
 
 // The same for two scores with |scale * s / softcap| <= 1/2 (`in` = scale / softcap, `out` = scale * log2(e)), from the
-// series of tanh: the first term left out is 21844/6081075 x^12 of the result, under 9e-7 of it.  Multiplies instead of the
-// two special-function instructions per score.
+// series of tanh: the first term left out is 21844/6081075 x^12 of the result, under 9e-7 of it, so the error is relative to
+// the score and does not know the cap.  Multiplies instead of the two special-function instructions per score.
 __device__ __forceinline__ float2 capped_small_scores(float2 s, float in, float out) {
   const float2 x = __fmul2_rn(s, make_float2(in, in)), y = __fmul2_rn(x, x);
   float2 t = make_float2(-1382.f / 155925.f, -1382.f / 155925.f);
@@ -145,6 +147,15 @@ __device__ __forceinline__ float2 capped_small_scores(float2 s, float in, float 
   t = __ffma2_rn(t, y, make_float2(-1.f / 3.f, -1.f / 3.f));
   t = __ffma2_rn(t, y, make_float2(1.f, 1.f));
   return __fmul2_rn(t, __fmul2_rn(s, make_float2(out, out)));
+}
+
+// Two scores under a cap above kTightCap, each by its own size, so that one huge score does not cost its neighbours their
+// digits.  Tight caps need only the logistic form: 460 against 542 us where most scores are past half a cap of 1 (4 chunks of
+// up to 1024 rows on 4096 tokens, 32 query / 8 KV heads, head_dim 128).
+__device__ __forceinline__ float2 capped_scores(float2 s, float in, float out, float e, float c) {
+  const float2 small = capped_small_scores(s, in, out);
+  return make_float2(fabsf(s.x * in) <= 0.5f ? small.x : capped_large_score(s.x, e, c),
+                     fabsf(s.y * in) <= 0.5f ? small.y : capped_large_score(s.y, e, c));
 }
 
 }  // namespace gk

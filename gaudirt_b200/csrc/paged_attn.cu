@@ -334,10 +334,22 @@ __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const
     // ---- scale, softcap, mask -----------------------------------------------------------
     const int tok0 = kv_begin + (warp + i * WARPS) * kGroupTokens;
     if (EXT && capped) {
+      const float in = p.scale / p.softcap, out = p.scale * kLog2e, twice = 2.f * kLog2e * in, cap = p.softcap * kLog2e;
+      if (p.softcap <= kTightCap) {
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+        for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[nt][e] = capped_score(sc[nt][e], 2.f * kLog2e * p.scale / p.softcap, p.softcap * kLog2e);
+          for (int e = 0; e < 4; ++e) sc[nt][e] = capped_large_score(sc[nt][e], twice, cap);
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const float2 v = capped_scores(make_float2(sc[nt][e], sc[nt][e + 1]), in, out, twice, cap);
+            sc[nt][e] = v.x;
+            sc[nt][e + 1] = v.y;
+          }
+      }
     } else {
       if (capped) {
         const float inv = p.scale / p.softcap;

@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
     const bool capped = BIASED || SHARED ? CAP : p.softcap > 0.f;
     const float to_log2 = capped ? kLog2e : p.scale * kLog2e;
     const float cap_in = capped ? p.scale / p.softcap : 0.f;
-    const float cap_exp = 2.f * kLog2e * cap_in, cap_log2 = p.softcap * kLog2e;     // see capped_score
+    const float cap_exp = 2.f * kLog2e * cap_in, cap_log2 = p.softcap * kLog2e;     // see capped_scores
     const bool steep = BIASED && __any_sync(0xffffffffu, fabsf(slope) * 31.f > 100.f);
     float m = -CUDART_INF_F, l = 0.f;                            // m: exponent reference of this row
     bool alive = true;
@@ -374,11 +374,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
                   r[e] = __float_as_uint((unsigned)(rel + c * 32 + e) <= (unsigned)span ? v.x : -CUDART_INF_F);
                   r[e + 1] = __float_as_uint((unsigned)(rel + c * 32 + e + 1) <= (unsigned)span ? v.y : -CUDART_INF_F);
                 }
+              } else if (capped && p.softcap > kTightCap) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                  float2 v = capped_scores(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), cap_in, p.scale * kLog2e, cap_exp, cap_log2);
+                  if (BIASED) {
+                    v.x = fmaf(-slope, fabsf(from + (float)(c * 32 + e)), v.x);
+                    v.y = fmaf(-slope, fabsf(from + (float)(c * 32 + e + 1)), v.y);
+                  }
+                  r[e] = __float_as_uint((unsigned)(rel + c * 32 + e) <= (unsigned)span ? v.x : -CUDART_INF_F);
+                  r[e + 1] = __float_as_uint((unsigned)(rel + c * 32 + e + 1) <= (unsigned)span ? v.y : -CUDART_INF_F);
+                }
               } else {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                   float v = __uint_as_float(r[e]);
-                  v = capped ? capped_score(v, cap_exp, cap_log2) : v * to_log2;
+                  v = capped ? capped_large_score(v, cap_exp, cap_log2) : v * to_log2;
                   if (BIASED) v = fmaf(-slope, fabsf(from + (float)(c * 32 + e)), v);
                   r[e] = __float_as_uint((unsigned)(rel + c * 32 + e) <= (unsigned)span ? v : -CUDART_INF_F);
                 }
