@@ -384,15 +384,17 @@ class PagedMetadata : public torch::CustomClassHolder {
                      device_status(device.index()).data_ptr<int32_t>(),
                      stream_of(at::cuda::getCurrentCUDAStream(device.index()))),
                  "device metadata");
-    check_shared_tables();
+    if (shared_pairs_.defined())
+      compare_tables(shared_pairs_, shared_verdict_, device_status(device.index()).data_ptr<int32_t>());
   }
 
   // Declares which sequences of the step begin with the same cached tokens in the same slots: sequence i is in group
   // `groups[i]` (-1 = none), and the first `prefix_tokens[g]` positions of every member of group g hold the same slots.
   // Plans built afterwards attend to such a prefix once for all rows of the group (where that pays); every attention
   // operator over this metadata then computes what it computed before.  Every member's new rows lie behind the prefix.
-  // The table rows are compared on the device and a difference is refused here (in `_revalidate_`: GK_DEV_BAD_METADATA
-  // in the status word); a table owned by the scheduler is vouched for by it.  Not part of the reference surface.
+  // The table rows are compared on the device and a difference is refused here, which leaves an earlier declaration and the
+  // status word as they were (in `_revalidate_`: GK_DEV_BAD_METADATA in the status word); a table owned by the scheduler
+  // is vouched for by it.  Not part of the reference surface.
   void share_prefixes_(std::vector<int64_t> groups, std::vector<int64_t> prefix_tokens) {
     const int64_t n_seq = static_cast<int64_t>(sequences_.size() / 4);
     TORCH_CHECK(plans_.empty(), "GaudiRT shared prefix: the metadata is already bound to an attention plan");
@@ -417,23 +419,21 @@ class PagedMetadata : public torch::CustomClassHolder {
         pairs.insert(pairs.end(), {sequences_[static_cast<size_t>(first[g]) * 4 + 3], seq[3], tokens[g], static_cast<int32_t>(i)});
       }
     }
+    at::Tensor device_pairs, verdict;
     if (!scheduler_owned_ && !pairs.empty()) {
       const auto device = locations_.device();
       c10::cuda::CUDAGuard guard(device);
       auto staging = at::empty({static_cast<int64_t>(pairs.size())}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
       std::memcpy(staging.data_ptr<int32_t>(), pairs.data(), pairs.size() * sizeof(int32_t));
-      shared_pairs_ = staging.to(device, /*non_blocking=*/true);
-      shared_verdict_ = at::empty({1}, at::TensorOptions().dtype(at::kInt).device(device));
-      check_shared_tables();
-      const int32_t bad = shared_verdict_.item<int32_t>();
-      if (bad != -1) {
-        clear_status_bits(device.index(), GK_DEV_BAD_METADATA);
-        shared_pairs_ = at::Tensor();
-        TORCH_CHECK(false, "GaudiRT shared prefix: sequence ", bad, " does not hold the slots of its group's prefix");
-      }
-    } else {
-      shared_pairs_ = at::Tensor();
+      device_pairs = staging.to(device, /*non_blocking=*/true);
+      verdict = at::empty({1}, at::TensorOptions().dtype(at::kInt).device(device));
+      compare_tables(device_pairs, verdict, nullptr);
+      const int32_t bad = verdict.item<int32_t>();
+      TORCH_CHECK(bad == -1, "GaudiRT shared prefix: sequence ", bad, " does not hold the slots of its group's prefix");
     }
+    // All of it or none: what was declared before stays in force, and compared, when this declaration is refused.
+    shared_pairs_ = std::move(device_pairs);
+    shared_verdict_ = std::move(verdict);
     shared_groups_ = std::move(group_of);
     shared_tokens_ = std::move(tokens);
   }
@@ -692,17 +692,14 @@ class PagedMetadata : public torch::CustomClassHolder {
       if (in[i]) in[i] = members[static_cast<size_t>(shared_groups_[i])] >= 2 && shared_tokens_[static_cast<size_t>(shared_groups_[i])] > 0;
     return in;
   }
-  // Compares the table rows of every group on the device; launches only.
-  void check_shared_tables() {
-    if (!shared_pairs_.defined()) return;
+  // Compares the declared table rows on the device (`verdict` receives the first sequence that differs); launches only.
+  void compare_tables(const at::Tensor& pairs, const at::Tensor& verdict, int32_t* status) const {
     const auto device = locations_.device();
     c10::cuda::CUDAGuard guard(device);
     check_status(gk_shared_prefix_check(mapping_.data_ptr<int32_t>(), mapping_.size(0), mapping_.size(1), mapping_.stride(0),
                                         batch_requests_.defined() ? batch_requests_.data_ptr<int32_t>() : nullptr,
                                         batch_requests_.defined() ? batch_requests_.numel() : mapping_.size(0),
-                                        shared_pairs_.data_ptr<int32_t>(), shared_pairs_.numel() / 4,
-                                        shared_verdict_.data_ptr<int32_t>(),
-                                        device_status(device.index()).data_ptr<int32_t>(),
+                                        pairs.data_ptr<int32_t>(), pairs.numel() / 4, verdict.data_ptr<int32_t>(), status,
                                         stream_of(at::cuda::getCurrentCUDAStream(device.index()))),
                  "shared prefix");
   }
