@@ -108,17 +108,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
                   batch <= 65536 && mapping.size(0) <= 262144,
               "GaudiRT paged allocator: unsupported page size, row count or request count");
   c10::cuda::CUDAGuard guard(device);
-  // One block for the six outputs: through the dispatcher one by one they cost the host as much as the launch.
-  const auto block = at::Tensor(at::detail::empty_cuda({(batch + 1) * 8 + (3 * rows + batch + 1) * 4}, at::kByte, device, c10::nullopt));
-  int64_t cursor = 0;
-  auto vector = [&](int64_t n, at::ScalarType type) {
-    const auto meta = at::scalarTypeToTypeMeta(type);
-    auto out = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), meta);
-    out.unsafeGetTensorImpl()->set_storage_offset(cursor / static_cast<int64_t>(meta.itemsize()));
-    out.unsafeGetTensorImpl()->set_sizes_contiguous({n});
-    cursor += n * static_cast<int64_t>(meta.itemsize());
-    return out;
-  };
+  // Each output is a tensor of its own, straight from the caching allocator: through the dispatcher the six of them cost the
+  // host as much as the launch.
+  auto vector = [&](int64_t n, at::ScalarType type) { return at::Tensor(at::detail::empty_cuda({n}, type, device, c10::nullopt)); };
   auto next_lengths = vector(batch, at::kLong), next_used = vector(1, at::kLong);
   auto locations = vector(rows, at::kInt), positions = vector(rows, at::kInt), row_requests = vector(rows, at::kInt);
   auto row_offsets = vector(batch + 1, at::kInt);
