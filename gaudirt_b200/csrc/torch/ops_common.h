@@ -431,7 +431,9 @@ class PagedMetadata : public torch::CustomClassHolder {
       const int32_t bad = verdict.item<int32_t>();
       TORCH_CHECK(bad == -1, "GaudiRT shared prefix: sequence ", bad, " does not hold the slots of its group's prefix");
     }
-    // All of it or none: what was declared before stays in force, and compared, when this declaration is refused.
+    // All of it or none: what was declared before stays in force, and compared, when this declaration is refused.  A graph
+    // that captured `_revalidate_` goes on comparing what was declared then: its list and verdict are kept as well.
+    if (shared_pairs_.defined()) earlier_pairs_.insert(earlier_pairs_.end(), {shared_pairs_, shared_verdict_});
     shared_pairs_ = std::move(device_pairs);
     shared_verdict_ = std::move(verdict);
     shared_groups_ = std::move(group_of);
@@ -672,6 +674,7 @@ class PagedMetadata : public torch::CustomClassHolder {
   int64_t last_plan_prefix_records_ = 0;
   std::vector<int32_t> shared_groups_, shared_tokens_, two_way_;   // per sequence, per group, per sequence
   at::Tensor shared_pairs_, shared_verdict_;                       // table rows that must agree, and the first that does not
+  std::vector<at::Tensor> earlier_pairs_;                          // those of declarations since replaced
   bool scheduler_owned_ = false;
   // Sequences of at most kSharedPackedRows packed rows whose groups are worth attending to together.
   static constexpr int64_t kSharedPackedRows = 64;

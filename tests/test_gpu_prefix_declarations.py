@@ -84,3 +84,26 @@ def test_a_refused_declaration_leaves_other_reports_standing(rt):
     with pytest.raises(RuntimeError, match="sequence 2 does not hold"):
         md._share_prefixes_([0, 0, 0], [160])
     assert rt._C._take_device_status() == 0
+
+
+def test_a_captured_comparison_outlives_its_declaration(rt):
+    """A graph that captured `_revalidate_` writes its verdict on every replay: into memory that is still its own after the
+    prefixes were declared anew."""
+    step, md, _ = device_step(rt)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        batch = torch.arange(3, dtype=torch.int32, device=DEV)
+        positions, locations = step.positions[:3].to(torch.int32).to(DEV), step.locations[:3].to(DEV)
+        md = rt.PagedMetadata.from_device(locations, batch, positions, step.mapping.to(DEV), step.cached[:3], step.lengths[:3],
+                                          step.slots)
+        md._share_prefixes_([0, 0, -1], [160])
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            md._revalidate_(locations, batch, positions)
+        md._share_prefixes_([-1, -1, -1], [])
+        held = [torch.full((4,), 7, dtype=torch.int32, device=DEV) for _ in range(2000)]
+        graph.replay()
+        stream.synchronize()
+        assert all(torch.equal(h, torch.full_like(h, 7)) for h in held)
+    assert rt._C._take_device_status() == 0
