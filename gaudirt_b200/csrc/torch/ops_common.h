@@ -507,7 +507,7 @@ class PagedMetadata : public torch::CustomClassHolder {
     // short chunks -- to the split-KV decode kernel.  Short chunks of a group that is attended to together stay with
     // its decode rows; a longer one reads the prefix once per 256 packed rows as it is and takes no part in the group.
     const int64_t min_saved = prefix_sharing_ > 0 ? 0 : shared_prefix_min_saved_bytes(head_dim);
-    const std::vector<char> together = short_group_members(query_heads, kv_heads, head_dim, min_saved);
+    const std::vector<char> together = short_group_members(query_heads, kv_heads, head_dim, window, min_saved);
     std::vector<int32_t> offered, offered_two_way, rest;
     for (int64_t i = 0; i < n_seq; ++i) {
       const int32_t* seq = &sequences_[static_cast<size_t>(i) * 4];
@@ -676,23 +676,28 @@ class PagedMetadata : public torch::CustomClassHolder {
   at::Tensor shared_pairs_, shared_verdict_;                       // table rows that must agree, and the first that does not
   std::vector<at::Tensor> earlier_pairs_;                          // those of declarations since replaced
   bool scheduler_owned_ = false;
-  // Sequences of at most kSharedPackedRows packed rows whose groups are worth attending to together.
+  // Sequences of at most kSharedPackedRows packed rows whose groups the plan attends to together: the saving is the plan's
+  // own (gk_shared_prefix_plan_build), so that no chunk leaves the prefill kernel for a group that is then not shared.
   static constexpr int64_t kSharedPackedRows = 64;
-  std::vector<char> short_group_members(int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t min_saved) const {
+  std::vector<char> short_group_members(int64_t query_heads, int64_t kv_heads, int64_t head_dim, int window, int64_t min_saved) const {
     if (shared_groups_.empty() || prefix_sharing_ == 0) return {};
+    struct Group { int64_t members = 0, low = INT32_MAX; };       // low: first key that any row of the group sees
+    std::vector<Group> group(shared_tokens_.size());
     std::vector<char> in(shared_groups_.size(), 0);
-    std::vector<int64_t> members(shared_tokens_.size(), 0);
     for (size_t i = 0; i < in.size(); ++i) {
       if (shared_groups_[i] < 0 || sequences_[i * 4 + 1] * (query_heads / kv_heads) > kSharedPackedRows) continue;
       in[i] = 1;
-      ++members[static_cast<size_t>(shared_groups_[i])];
+      Group& g = group[static_cast<size_t>(shared_groups_[i])];
+      ++g.members;
+      g.low = std::min<int64_t>(g.low, window > 0 ? std::max(0, sequences_[i * 4 + 2] - window + 1) : 0);
     }
+    auto seen = [&](size_t g) { return group[g].members >= 2 ? std::max<int64_t>(0, shared_tokens_[g] - group[g].low) : 0; };
     int64_t saved = 0;
-    for (size_t g = 0; g < members.size(); ++g)
-      if (members[g] >= 2) saved += (members[g] - 1) * shared_tokens_[g] * kv_heads * head_dim * 4;
+    for (size_t g = 0; g < group.size(); ++g)
+      if (seen(g) > 0) saved += (group[g].members - 1) * seen(g) * kv_heads * head_dim * 4;
     if (saved < min_saved) return {};
     for (size_t i = 0; i < in.size(); ++i)
-      if (in[i]) in[i] = members[static_cast<size_t>(shared_groups_[i])] >= 2 && shared_tokens_[static_cast<size_t>(shared_groups_[i])] > 0;
+      if (in[i]) in[i] = seen(static_cast<size_t>(shared_groups_[i])) > 0;
     return in;
   }
   // Compares the declared table rows on the device (`verdict` receives the first sequence that differs); launches only.

@@ -107,3 +107,54 @@ def test_a_captured_comparison_outlives_its_declaration(rt):
         stream.synchronize()
         assert all(torch.equal(h, torch.full_like(h, 7)) for h in held)
     assert rt._C._take_device_status() == 0
+
+
+def draft_metadata(rt, groups, prefixes, behind, rows, page=128):
+    """Sequences of `rows` new rows each, `behind` cached tokens behind the prefix of their group."""
+    starts = [prefixes[g] if g >= 0 else 0 for g in groups]
+    ends = [s + b + rows for s, b in zip(starts, behind)]
+    table = torch.full((len(groups), max(ends)), -1, dtype=torch.int32)
+    at = 0
+    heads = []
+    for p in prefixes:
+        heads.append(torch.arange(at, at + p, dtype=torch.int32))
+        at += -(-p // page) * page
+    for i, (g, s, e) in enumerate(zip(groups, starts, ends)):
+        if g >= 0:
+            table[i, :s] = heads[g]
+        table[i, s:e] = torch.arange(at, at + e - s, dtype=torch.int32)
+        at += -(-(e - s) // page) * page
+    requests = torch.arange(len(groups)).repeat_interleave(rows)
+    positions = torch.cat([torch.arange(e - rows, e) for e in ends])
+    return rt.PagedMetadata(table[requests, positions].contiguous(), requests, positions, table, at)
+
+
+# cached tokens behind the prefix, window: nobody sees the prefix; a piece of it that is not worth a launch of its own
+@pytest.mark.parametrize("behind,window", [(300, 256), (100, 256), (0, 1)])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_a_window_that_hides_the_prefix_leaves_the_plan_alone(rt, head_dim, behind, window):
+    """Short chunks stay where they are when their group is not attended to together: the records are those of a step
+    without declarations."""
+    plans = []
+    for declared in (False, True):
+        md = draft_metadata(rt, [0] * 24, [16384], [behind] * 24, 12)
+        if declared:
+            md._share_prefixes_([0] * 24, [16384])
+        plans.append(md.attention_plan_for(32, 8, head_dim, window))
+        assert md._last_plan_prefix_records() == 0
+    assert torch.equal(*plans)
+
+
+def test_only_groups_that_are_seen_are_taken_together(rt):
+    """Two groups under one window: one sees its prefix and is shared, the other does not and keeps the records it had."""
+    groups = [0] * 24 + [1] * 4
+    behind = [0] * 24 + [5000] * 4
+    md = draft_metadata(rt, groups, [16384, 4096], behind, 12)
+    md._share_prefixes_(groups, [16384, 4096])
+    md._set_prefix_sharing(1, 0)
+    both = md.attention_plan_for(32, 8, 128, 4096)
+    assert md._last_plan_prefix_records() > 0
+    md = draft_metadata(rt, groups, [16384, 4096], behind, 12)
+    md._share_prefixes_([0] * 24 + [-1] * 4, [16384])
+    md._set_prefix_sharing(1, 0)
+    assert torch.equal(both, md.attention_plan_for(32, 8, 128, 4096))
