@@ -1,5 +1,6 @@
 // Host side of the C ABI: status text, pool geometry, paged-metadata validation and the
-// length-aware split-KV schedule.  Nothing here touches the device.
+// length-aware split-KV schedule.  Nothing here touches the device, and nothing leaves a C entry by exception: lists that do
+// not fit into memory end as GK_ERR_CAPACITY.
 #include "../../include/gaudirt_b200.h"
 
 #include <algorithm>
@@ -9,12 +10,11 @@
 #include <functional>
 #include <cstdint>
 #include <numeric>
-#include <string>
 #include <unordered_map>
 #include <vector>
 
 namespace {
-thread_local std::string g_metadata_error;
+thread_local const char* g_metadata_error = "";     // always one of the messages below: nothing is allocated
 
 int metadata_fail(const char* message) {
   g_metadata_error = message;
@@ -42,7 +42,7 @@ extern "C" const char* gk_status_string(int status) {
 
 extern "C" int gk_abi_version(void) { return 1; }
 extern "C" int gk_last_cuda_error(void) { return gk::g_last_cuda_error; }
-extern "C" const char* gk_metadata_error(void) { return g_metadata_error.c_str(); }
+extern "C" const char* gk_metadata_error(void) { return g_metadata_error; }
 
 extern "C" int gk_paged_kv_pool_bytes(int64_t layers, int64_t slots, int64_t kv_heads, int64_t head_dim,
                                       uint64_t* bytes_out) {
@@ -61,7 +61,7 @@ extern "C" int gk_paged_kv_pool_bytes(int64_t layers, int64_t slots, int64_t kv_
 extern "C" int gk_paged_metadata_validate(const int32_t* locations, const int32_t* requests, const int32_t* positions,
                                           int64_t rows, const int32_t* mapping, int64_t n_requests, int64_t context,
                                           int64_t slots, int32_t* seq_out, int64_t* n_seq_out,
-                                          int32_t* page_tokens_out) {
+                                          int32_t* page_tokens_out) try {
   if (!locations || !requests || !positions || !mapping || !seq_out || !n_seq_out) return GK_ERR_INVALID_ARGUMENT;
   if (rows <= 0 || rows > INT32_MAX || slots <= 0 || slots > INT32_MAX || n_requests <= 0 || n_requests > INT32_MAX ||
       context <= 0 || context > INT32_MAX || n_requests * context > INT32_MAX)
@@ -117,6 +117,8 @@ extern "C" int gk_paged_metadata_validate(const int32_t* locations, const int32_
   *n_seq_out = n_seq;
   if (page_tokens_out) *page_tokens_out = page;
   return GK_OK;
+} catch (...) {
+  return GK_ERR_CAPACITY;
 }
 
 // Host half of slot allocation (src/bridge/paged_slot_allocator.cpp:95-128): the argument checks
@@ -377,9 +379,11 @@ int attention_plan_build(const int32_t* seq, int64_t n_seq, const SequenceExtras
 extern "C" int gk_attention_plan_build(const int32_t* seq, int64_t n_seq, int q_heads, int kv_heads, int head_dim,
                                        int window, int sm_count, int split_tokens, int32_t* work_out,
                                        int64_t work_cap, int64_t* n_work_out, int32_t* combine_out,
-                                       int64_t combine_cap, int64_t* n_combine_out, int64_t* partial_entries_out) {
+                                       int64_t combine_cap, int64_t* n_combine_out, int64_t* partial_entries_out) try {
   return attention_plan_build(seq, n_seq, SequenceExtras{}, q_heads, kv_heads, head_dim, window, sm_count, split_tokens,
                               work_out, work_cap, n_work_out, combine_out, combine_cap, n_combine_out, partial_entries_out);
+} catch (...) {
+  return GK_ERR_CAPACITY;
 }
 
 // Sequences whose rows see a two-way prefix and, by group, read a common prefix together.
@@ -574,7 +578,7 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
   }
   return GK_OK;
 } catch (...) {
-  return GK_ERR_CAPACITY;     // the lists of a plan did not fit into memory; nothing leaves a C entry by exception
+  return GK_ERR_CAPACITY;
 }
 
 namespace {
@@ -630,9 +634,11 @@ int prefill_plan_build(const int32_t* seq, int64_t n_seq, const int32_t* two_way
 
 extern "C" int gk_prefill_plan_build(const int32_t* seq, int64_t n_seq, int q_heads, int kv_heads, int window,
                                      int min_rows, int32_t* work_out, int64_t work_cap, int64_t* n_work_out,
-                                     int32_t* rest_seq_out, int64_t* n_rest_out) {
+                                     int32_t* rest_seq_out, int64_t* n_rest_out) try {
   return prefill_plan_build(seq, n_seq, nullptr, q_heads, kv_heads, window, min_rows, work_out, work_cap, n_work_out,
                             rest_seq_out, n_rest_out);
+} catch (...) {
+  return GK_ERR_CAPACITY;
 }
 
 extern "C" int gk_prefill_plan_build_two_way(const int32_t* seq, int64_t n_seq, const int32_t* two_way, int q_heads,

@@ -50,7 +50,7 @@ enum gk_status {
   GK_ERR_INVALID_ARGUMENT = 1,  /* null pointer, negative size, misaligned pointer or stride   */
   GK_ERR_UNSUPPORTED = 2,       /* geometry outside what the kernels implement: fail fast      */
   GK_ERR_CUDA = 3,              /* the CUDA runtime refused the launch; see gk_last_cuda_error */
-  GK_ERR_CAPACITY = 4,          /* an output array or fixed scratch area is too small          */
+  GK_ERR_CAPACITY = 4,          /* an output array, a scratch area or host memory is too small  */
   GK_ERR_METADATA = 5           /* host metadata validation failed; see the message accessor   */
 };
 
