@@ -30,12 +30,6 @@ torch.ops.load_library(build.OPS_SO)
 
 PagedMetadata = torch.classes.gaudirt.PagedMetadata
 
-# Every operator call looks for a `__torch_function__` on its arguments.  A script object such as PagedMetadata has none, and
-# the search that fails builds and discards a C++ exception: half of the 19 us that an attention call cost the host.  Saying
-# on the class what is the case -- script objects do not override torch functions -- ends the search at once.
-if "__torch_function__" not in vars(torch.ScriptObject):
-    torch.ScriptObject.__torch_function__ = torch._C._disabled_torch_function_impl
-
 _C = types.SimpleNamespace(
     _allocate_paged_kv=lambda layers, slots, heads, head_dim: torch.ops.gaudirt._allocate_paged_kv(
         layers, slots, heads, head_dim),
