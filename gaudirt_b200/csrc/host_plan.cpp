@@ -408,7 +408,7 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
   const int tile_rows = GK_PREFILL_TILE_ROWS / group_heads;
   const int ctas_per_record = head_dim == 256 ? 2 : 1;
 
-  struct Group { std::vector<int32_t> members; int64_t rows = 0; int32_t lo = 0, hi = 0; };
+  struct Group { std::vector<int32_t> members; int64_t rows = 0; int32_t lo = 0, hi = 0, seen = 0; };
   std::vector<Group> all(static_cast<size_t>(n_groups));
   int64_t last_row = 0;
   for (int64_t s = 0; s < n_seq; ++s) {
@@ -434,7 +434,8 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
       one.lo = std::min(one.lo, window > 0 ? std::max(0, seq[s * 4 + 2] - window + 1) : 0);   // first key any row sees
     if (one.members.size() < 2 || one.hi <= one.lo) continue;
     saved += (int64_t)(one.members.size() - 1) * (one.hi - one.lo) * token_bytes;
-    one.lo = one.lo / tile * tile;                                   // whole tiles: a row's own window is masked in the kernel
+    one.seen = one.lo;
+    one.lo = one.lo / tile * tile;      // cut at whole tiles; the first record says where its keys begin, the kernel masks a row's own window
     shared.push_back(&one);
   }
   if (saved < min_saved_bytes) shared.clear();
@@ -539,7 +540,7 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
       int32_t highest = 0;
       for (int32_t i = 0; i < n; ++i) highest = std::max(highest, places[at + i][1]);
       for (int64_t part = 0; part < parts; ++part)
-        items.push_back({{(int32_t)(rows.size()), n, (int32_t)part, seq[g->members[0] * 4 + 3], (int32_t)(g->lo + part * even),
+        items.push_back({{(int32_t)(rows.size()), n, (int32_t)part, seq[g->members[0] * 4 + 3], std::max(g->seen, (int32_t)(g->lo + part * even)),
                           (int32_t)std::min<int64_t>(g->hi, g->lo + (part + 1) * even), highest, 0}});
       for (int32_t i = 0; i < n; ++i) rows.push_back({places[at + i][0], places[at + i][1], 0, 0});
     }

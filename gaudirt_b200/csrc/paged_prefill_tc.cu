@@ -194,6 +194,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
   }
   const int rows0 = min(n_rows, tile_rows), rows1 = NARROW ? rows0 : n_rows - rows0;
   const int tile_step = NARROW ? 0 : tile_rows;             // rows between the two tiles (chains)
+  // The first record of a shared prefix may begin inside a tile (the first key that any of its rows' windows shows): its
+  // tiles stay on the pool's boxes, and what lies in front of it is zeros like what lies behind kv_end.
+  const int kv_seen = kv_begin;
+  if (SHARED) kv_begin = kv_begin / kKv * kKv;
   // KV tiles each query tile needs: tile 0 stops at its own last row (causal), tile 1 at the record's end
   const int nt1_all = (kv_end - kv_begin + kKv - 1) / kKv;
   const int nt0 = NARROW ? (nt1_all + 1) / 2 : SHARED ? nt1_all : min(nt1_all, (last_seen(first_row + rows0 - 1, first_pos + rows0 - 1) + 1 - kv_begin + kKv - 1) / kKv);
@@ -646,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const Pre
       for (int half = 0; half < kHalves; ++half) {
         const int tok = tile_at(j) + lwarp * kWarpRows + half * 32 + lane;
         slot[half] = -1;
-        if (tok < kv_end) {
+        if (tok < kv_end && (!SHARED || tok >= kv_seen)) {
           slot[half] = __ldg(trow + (int64_t)(tok >> p.page_shift) * p.entry_stride) + (tok & page_mask);
           if ((unsigned)slot[half] >= (unsigned)p.slots) {
             if (p.status) atomicOr(p.status, (int)GK_DEV_BAD_TABLE);
