@@ -441,7 +441,7 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
   if (saved < min_saved_bytes) shared.clear();
   // The form of the records (one or two query tiles) and how long a piece of the prefix one CTA takes: the cheapest by a
   // model of the two kernels side by side, in us.  A prefix CTA has an SM to itself for a fixed 7 us and 1.2 us per 128 keys
-  // and one query tile, 2.4 us per two (1.0 and 1.9 at head_dim 64, 1.1 per 64 keys at 256).  The members' own CTAs take
+  // and one query tile, 2.4 us per two (1.0 and 1.9 at head_dim 64, 1.1 per 64 keys at 256; scores without cap or bias).  The members' own CTAs take
   // 3.5 us and 36 GB/s each, two per SM on the SMs that the prefix leaves and on all of them once it is done, never faster
   // than memory gives their bytes and never more than 50 of them in a us (2048 of 64 KB took 40 us on 84 and on 148 SMs).  Every part of a row costs its merge 0.15 us.  So the longer of the two
   // gets the SMs: measured with 256 members of 4096 + 1024 tokens, 32 CTAs of two tiles or 64 of one 108 us, 128 of one
@@ -557,7 +557,8 @@ extern "C" int gk_shared_prefix_plan_build(const int32_t* seq, int64_t n_seq, co
   if (built != GK_OK) return built;
   // Tails of one query block each, many of them and short: two warps and four CTAs per SM instead of four warps and two,
   // so that a CTA's fixed cost (3 to 4 us of look-ups and merges) is a smaller part of its time.  Measured at head_dim 128:
-  // 10-14 % faster at 1024 and 2048 CTAs of 64 to 512 tokens, even at 8192 tokens, 10-25 % slower at 128 to 512 CTAs.
+  // 10-14 % faster at 1024 and 2048 CTAs of 64 to 512 tokens, even at 8192 tokens, 10-25 % slower at 128 to 512 CTAs; all
+  // of that with few prefix CTAs beside them, so the rule counts every SM and not the ones that the prefix leaves.
   int64_t own_tokens = 0;
   for (int64_t s = 0; s < n_seq; ++s) own_tokens += seq[s * 4 + 2] + seq[s * 4 + 1] - kv_from[s];
   const bool short_tails = head_dim != 256 && !items.empty() && *n_work_out * kv_heads >= 6 * (int64_t)sm_count &&

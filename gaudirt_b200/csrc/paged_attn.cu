@@ -86,7 +86,8 @@ __device__ __forceinline__ uint32_t group_off(int row, int chunk) {
 
 // EXT: distance bias, row limits and the launch beside a shared-prefix kernel; without it none of the three costs an
 // instruction.  The bias is one fused multiply-add per score and hides behind the K/V stream: 64 rows on contexts up to 8192
-// (1.11 GB of K/V, 32 query / 8 KV heads) take 162 us, 6.9 TB/s.
+// (1.11 GB of K/V, 32 query / 8 KV heads, another pool each time) take 163 us in a replayed graph and 164 us called pass after
+// pass, 6.8 TB/s: the rate of reads alone, which is above that of a copy.
 template <int D, int WARPS, int STAGES, bool TMA, bool EXT>
 __global__ void __launch_bounds__(WARPS * 32, 8 / WARPS) paged_attn_kernel(const AttnParams p,
                                                                    const __grid_constant__ CUtensorMap map_kv) {
