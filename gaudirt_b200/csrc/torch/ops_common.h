@@ -56,9 +56,6 @@ inline std::atomic<bool>& fuse_kv_store_flag() {
 }
 inline bool fuse_kv_store() { return fuse_kv_store_flag().load(std::memory_order_relaxed); }
 
-// Clears `bits` of the device status word, in stream order: for errors that were raised on the host.
-inline void clear_status_bits(c10::DeviceIndex device, int bits) { device_status(device).bitwise_and_(~bits); }
-
 // ---------------------------------------------------------------------------------------------
 // attention plan carried by its device tensor (as in src/bridge/attention_plan.cpp:132-140,
 // 319-322: the tensor's storage context owns the host-side schedule, so the tensor's lifetime
@@ -264,6 +261,9 @@ class PagedMetadata : public torch::CustomClassHolder {
     const int wide = (loc.scalar_type() == at::kLong ? 1 : 0) | (req.scalar_type() == at::kLong ? 2 : 0) |
                      (pos.scalar_type() == at::kLong ? 4 : 0) | (has_tokens && tok.scalar_type() == at::kLong ? 8 : 0);
     const auto stream = at::cuda::getCurrentCUDAStream(device.index());
+    // A verdict that is read back below is an error of this call, not a report for the end of the step.  The word itself is
+    // made here all the same: a captured `_revalidate_` must not be its first use.
+    int32_t* status_word = device_status(device.index()).data_ptr<int32_t>();
     check_status(gk_paged_metadata_device_validate(
                      loc.data_ptr(), req.data_ptr(), pos.data_ptr(), has_tokens ? tok.data_ptr() : nullptr, wide,
                      vocabulary, scheduler_owned ? nullptr : mapping.data_ptr<int32_t>(), mapping.size(0), context,
@@ -272,7 +272,7 @@ class PagedMetadata : public torch::CustomClassHolder {
                      has_tokens ? token_ids_.data_ptr<int32_t>() : nullptr, last_token_indices_.data_ptr<int32_t>(),
                      row_status.data_ptr<int32_t>(), has_tokens ? token_status.data_ptr<int32_t>() : nullptr,
                      reinterpret_cast<uint64_t*>(verdict.data_ptr<int64_t>()),
-                     device_status(device.index()).data_ptr<int32_t>(), stream_of(stream)),
+                     scheduler_owned ? status_word : nullptr, stream_of(stream)),
                  "device metadata");
     dev_seq_ = seq_device;
     dev_workspace_ = workspace;
@@ -287,7 +287,6 @@ class PagedMetadata : public torch::CustomClassHolder {
       // entry per page and the prefill kernel may fetch whole pages by TMA.
       const uint64_t page = static_cast<uint64_t>(host.data_ptr<int64_t>()[2]);
       page_tokens_ = static_cast<int64_t>(std::min<uint64_t>(page, 128));
-      if (first != UINT64_MAX || token != UINT64_MAX) clear_status_bits(device.index(), GK_DEV_BAD_METADATA);
       uint64_t bad_row = first >> 8, bad_code = first & 255;
       if (first != UINT64_MAX && bad_code == 4) {
         // Two rows write one slot: on the device, which of them met the other's mark depends on arrival
